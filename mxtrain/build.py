@@ -41,6 +41,8 @@ HIP_FLAGS = [
     "-fvisibility=hidden",
     "-ffp-contract=fast",
     "-Wno-unused-result",
+    # no packed fp32 math (v_pk_add / mul / fma_f32): scalar forms only, rounding unchanged
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 
 
@@ -75,7 +77,7 @@ def build_kernels(jobs: int = 8, verbose: bool = False) -> str:
     for s in srcs:
         o = os.path.join(OBJDIR, os.path.basename(s) + ".o")
         objs.append(o)
-        if _newer([s] + hdrs, o):
+        if _newer([s, os.path.abspath(__file__)] + hdrs, o):   # (a change of flags rebuilds too)
             todo.append((s, o))
 
     def compile_one(so):
