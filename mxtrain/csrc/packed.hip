@@ -1,0 +1,690 @@
+// Packed causal attention for gfx950: sequences of different lengths laid end to end on one
+// token axis, grouped heads, forward and atomics-free backward.
+//
+//   s_ij = scale q_i . k_j   for start(i) <= j <= i,   p_i = softmax_j(s_ij),   o_i = sum_j p_ij v_j
+//   ds_ij = p_ij (do_i . v_j - delta_i),  delta_i = do_i . o_i
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i
+//
+// start(t) / end(t) are the bounds of the sequence of row t (packed_plan_kernel, from the
+// cumulative lengths).  The kernels tile the PACKED axis, not each sequence: a 128-row block
+// takes the keys [start(first row), last row], so a block may hold the end of one sequence and
+// the beginning of others and many short sequences cost no padding; a 32 x 32 subtile is skipped,
+// taken whole, or masked per element (start(i) <= j <= i is one unsigned compare).  Rows behind
+// the last sequence (a batch padded to a fixed size) are never read.
+//
+// A masked score has p = 0, but 0 * NaN = NaN inside a matrix product: a masked subtile whose
+// V (dQ: K; dK / dV: Q, dO) rows hold a non-finite value marks its wave, and the wave's rows are
+// redone one by one over their visible terms alone, so one sequence's infinities and NaN never
+// reach another's rows, nor a later row's an earlier one.
+#include "flash_common.h"
+#include "gemm_common.h"
+
+#include <type_traits>
+
+using namespace mx;
+using namespace mx::flash;
+using mx::gemm::buffer_rsrc;
+using mx::gemm::i32x4_t;
+
+namespace {
+
+// ------------------------------------------------------------------------------ plan
+// start / end / position of every row from the cumulative lengths cu[0..n] (one binary search per
+// row: the last i with cu[i] <= t, so sequences of length zero are passed over).  Every value is
+// clamped into [0, T], so a table that breaks its contract gives wrong sequences, never an access
+// out of range.  meta[0] = rows that belong to a sequence.  Rows behind them: start = end = t.
+template <typename IT>
+__global__ __launch_bounds__(256) void packed_plan_kernel(const IT* __restrict__ cu, int n, int T,
+                                                          int* __restrict__ start, int* __restrict__ end,
+                                                          int* __restrict__ meta, int64_t* __restrict__ pos) {
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  const long long last = (long long)cu[n];
+  const int nv = (int)(last < 0 ? 0 : last > T ? T : last);
+  if (t == 0) meta[0] = nv;
+  if (t >= T) return;
+  int s = t, e = t;
+  if (t < nv) {
+    int lo = 0, hi = n;   // cu[lo] <= t < cu[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((long long)cu[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    const long long a = (long long)cu[lo], b = (long long)cu[lo + 1];
+    s = (int)(a < 0 ? 0 : a > t ? t : a);
+    e = (int)(b < t + 1 ? t + 1 : b > nv ? nv : b);
+  }
+  start[t] = s;
+  end[t] = e;
+  pos[t] = t - s;
+}
+
+struct PArgs {
+  const uint16_t *q, *k, *v, *dout, *o;
+  uint16_t *out, *dk, *dv;      // forward: O; backward: dQ, dK, dV
+  float *lse, *delta;           // [Hq][T]
+  const int *start, *end, *meta;
+  int ldq, ldk, ldv, lddo, ldo, ldout, lddk, lddv;
+  int T, Hq, Hkv;
+  float c, scale;               // scale log2(e), scale
+  int fill;                     // zero the rows behind the last sequence (else leave them)
+};
+
+__device__ __forceinline__ uint32_t nonfinite(bf16x8 x) {   // high bit set in a half whose exponent is all ones
+  const uint4 u = __builtin_bit_cast(uint4, x);
+  constexpr uint32_t M = 0x7f807f80u, A = 0x00800080u;
+  return (((u.x & M) + A) | ((u.y & M) + A) | ((u.z & M) + A) | ((u.w & M) + A)) & 0x80008000u;
+}
+
+// Row-at-a-time forms for a wave whose masked subtiles met a non-finite operand: every lane holds
+// columns lane (+ 64) of the row, and only visible terms are ever formed.
+template <int D>
+struct RowVec {
+  float x[D / 64];
+  __device__ __forceinline__ RowVec() {
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) x[i] = 0.f;
+  }
+  __device__ __forceinline__ RowVec(const uint16_t* p, int lane) {
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) x[i] = bf2f(p[lane + 64 * i]);
+  }
+  __device__ __forceinline__ float dot(const RowVec& y) const {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) s += x[i] * y.x[i];
+    return wave_sum(s);
+  }
+  __device__ __forceinline__ void axpy(float w, const RowVec& y) {
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) x[i] = __builtin_fmaf(w, y.x[i], x[i]);
+  }
+  __device__ __forceinline__ void store(uint16_t* p, int lane, float sc) const {
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) p[lane + 64 * i] = f2bf(x[i] * sc);
+  }
+};
+
+// one 1-KiB LDS-DMA piece through a buffer resource: rows past its size read zeros
+__device__ __forceinline__ void dma16_buf(i32x4_t rsrc, uint32_t voff, char* lds_base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               :: "v"(voff), "s"(rsrc), "s"(lds_u32(lds_base)) : "memory", "m0");
+}
+// resource over `rows` rows of D values at `base` (row stride ld); rows <= 0: everything reads zero
+template <int D>
+__device__ __forceinline__ i32x4_t rows_rsrc(const uint16_t* base, int rows, int ld) {
+  const uint64_t b = (uint64_t)(uintptr_t)base;
+  const uint32_t bytes = rows > 0 ? ((uint32_t)(rows - 1) * (uint32_t)ld + D) * 2u : 0u;
+  return i32x4_t{uni((int)(uint32_t)b), uni((int)(uint32_t)(b >> 32)), uni((int)bytes), 0x00020000};
+}
+
+template <int D>
+__device__ __forceinline__ void zero_row(uint16_t* row, int hh) {   // the lane's half of a D-wide row
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) *reinterpret_cast<uint4*>(row + 16 * i + 8 * hh) = make_uint4(0, 0, 0, 0);
+}
+
+// ============================================================================ query-major
+// Forward, and dQ of the backward.  Four waves of 32 query rows; query on the MFMA lane
+// (S^T = K Q^T, O^T = V^T P^T), so the softmax statistics are lane-local plus one half exchange.
+// K / V tiles of BK keys arrive by LDS-DMA into a two-slot ring, one barrier per tile.
+template <int D, bool DQ>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void packed_qmajor_kernel(const PArgs a) {
+  constexpr int BQ = 128, BK = D == 64 ? 128 : 64, NSUB = BK / 32, NKK = D / 16, NDT = D / 32;
+  constexpr int RB = D * 2, CPR = D / 8, RPP = 64 / CPR, TILE = BK * RB, PPW = TILE / 1024 / 4;
+  __shared__ __attribute__((aligned(16))) char kbuf0[TILE];
+  __shared__ __attribute__((aligned(16))) char kbuf1[TILE];
+  __shared__ __attribute__((aligned(16))) char vbuf0[TILE];
+  __shared__ __attribute__((aligned(16))) char vbuf1[TILE];
+  const int tid = threadIdx.x, lane = tid & 63, wl = uni(tid >> 6);
+  const int r = lane & 31, hh = lane >> 5, g = lane >> 4, gi = lane & 15;
+  const int T = a.T, nqb = (T + BQ - 1) / BQ;
+  const int nv = uni(a.meta[0]);
+  int rank, hq;
+  block_map(a.Hq, rank, hq);
+  const int hk = hq / (a.Hq / a.Hkv);
+  const int q0 = (nqb - 1 - rank) * BQ;              // late blocks (most keys of a long sequence) first
+  const int qw = q0 + 32 * wl, qrow = qw + r;
+  uint16_t* outp = a.out + (size_t)qrow * a.ldout + hq * D;
+  if (q0 >= nv) {                                    // behind the last sequence
+    if (a.fill && qrow < T) {
+      zero_row<D>(outp, hh);
+      if (!DQ && hh == 0) a.lse[(size_t)hq * T + qrow] = INFINITY;
+    }
+    return;
+  }
+  const int q_end = min(q0 + BQ, nv);
+  const int kv_lo = uni(a.start[q0]) & ~31;
+  const int ntile = (q_end - kv_lo + BK - 1) / BK;
+  // the wave's rows: visible keys of row i are start(i) .. i
+  const bool wave_on = qw < nv;
+  const int wlast = min(qw + 31, nv - 1);
+  const int smin = uni(a.start[min(qw, nv - 1)]), smax = uni(a.start[wlast]);
+  const int qrow_c = min(qrow, nv - 1);
+  const int st = a.start[qrow_c];
+  const int cnt = qrow < nv ? qrow - st + 1 : 0;     // visible keys
+
+  bf16x8 qf[NKK];
+  bf16x8 dof[DQ ? NKK : 1];
+  float lse2 = 0.f, dl = 0.f;
+  {
+    const uint16_t* qp = a.q + (size_t)qrow_c * a.ldq + hq * D + 8 * hh;
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) qf[kk] = ld8(qp + 16 * kk);
+    if constexpr (DQ) {
+      const uint16_t* dp = a.dout + (size_t)qrow_c * a.lddo + hq * D + 8 * hh;
+      const uint16_t* op = a.o + (size_t)qrow_c * a.ldo + hq * D + 8 * hh;
+      float s = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk) {
+        dof[kk] = ld8(dp + 16 * kk);
+        float x[8], y[8];
+        unpack8(__builtin_bit_cast(uint4, dof[kk]), x);
+        unpack8(*reinterpret_cast<const uint4*>(op + 16 * kk), y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += x[j] * y[j];
+      }
+      dl = xhalf_sum(s);
+      lse2 = a.lse[(size_t)hq * T + qrow_c];
+      if (hh == 0 && qrow < nv) a.delta[(size_t)hq * T + qrow] = dl;   // read by the dK / dV kernel
+    }
+  }
+  float m_i = -INFINITY, l_i = 0.f;
+  f32x16 acc[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) acc[dt] = f32x16{};
+  // row operands complete before the loop, through the compiler-visible wait: it does not count
+  // the DMA issued from asm, and would wait for these loads in front of the loop's MFMAs
+  __builtin_amdgcn_s_waitcnt(0);
+
+  int offK[NKK];
+#pragma unroll
+  for (int kk = 0; kk < NKK; ++kk) offK[kk] = toff<D>(r, 2 * kk + hh);
+  int offT[NDT][2];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) {
+    const int col = 32 * dt + 16 * (g & 1) + 4 * (gi & 3), row0 = 4 * hh + (gi >> 2);
+    offT[dt][0] = toff<D>(row0, col >> 3) + (col & 7) * 2;
+    offT[dt][1] = toff<D>(row0 + 8, col >> 3) + (col & 7) * 2;
+  }
+  uint32_t voK[PPW], voV[PPW];
+#pragma unroll
+  for (int i = 0; i < PPW; ++i) {
+    const int R = (wl + 4 * i) * RPP + lane / CPR, ch = (lane % CPR) ^ swz<D>(R);
+    voK[i] = (uint32_t)(R * a.ldk + ch * 8) * 2u;
+    voV[i] = (uint32_t)(R * a.ldv + ch * 8) * 2u;
+  }
+  const uint16_t* kbase = a.k + (size_t)kv_lo * a.ldk + hk * D;
+  const uint16_t* vbase = a.v + (size_t)kv_lo * a.ldv + hk * D;
+  auto issue = [&](char* kd, char* vd, int j) __attribute__((always_inline)) {
+    const int rows = min(BK, nv - kv_lo - j * BK);
+    const i32x4_t kr = rows_rsrc<D>(kbase + (size_t)j * BK * a.ldk, rows, a.ldk);
+    const i32x4_t vr = rows_rsrc<D>(vbase + (size_t)j * BK * a.ldv, rows, a.ldv);
+#pragma unroll
+    for (int i = 0; i < PPW; ++i) {
+      dma16_buf(kr, voK[i], kd + (wl + 4 * i) * 1024);
+      dma16_buf(vr, voV[i], vd + (wl + 4 * i) * 1024);
+    }
+  };
+  const float c = a.c;
+
+  auto seen = [&](int k0, int e) __attribute__((always_inline)) {   // key k0 + crow(e, hh) visible to the lane's row
+    return (uint32_t)(k0 + 4 * hh - st + crow(e, 0)) < (uint32_t)cnt;
+  };
+  auto scores = [&](const char* Kt) __attribute__((always_inline)) {
+    f32x16 s = f32x16{};
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) s = mfma32(lds8(Kt, offK[kk]), qf[kk], s);
+    return s;
+  };
+  auto raise_max = [&](float mx) __attribute__((always_inline)) {
+    mx = xhalf_max(mx);
+    if (!__all(mx <= m_i)) {               // some row raised its maximum
+      const float m_new = fmaxf(m_i, mx);
+      const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_i - m_new) * c);
+      l_i *= alpha;
+      m_i = m_new;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[dt][e] *= alpha;
+    }
+    return m_i == -INFINITY ? 0.f : m_i * c;
+  };
+  auto expo = [&](f32x16& s, float mc) __attribute__((always_inline)) {   // s -> P, row sums into l_i
+    float rs0 = 0.f, rs1 = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -mc));
+      s[e + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], c, -mc));
+      rs0 += s[e];
+      rs1 += s[e + 1];
+    }
+    l_i += rs0 + rs1;
+  };
+  auto tfrag = [&](const char* Xt, int h, int dt) __attribute__((always_inline)) {   // 32 columns of d x 16 rows
+    return cat(tr_read(Xt + 16 * h * RB, offT[dt][0]), tr_read(Xt + 16 * h * RB, offT[dt][1]));
+  };
+  // acc += (weights w of the 32 rows) X, w rounded to bf16 for the matrix unit (sums stay fp32)
+  auto accum = [&](const char* Xt, const f32x16& w) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bf16x8 wb = pack8(w, 8 * h);
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) acc[dt] = mfma32(tfrag(Xt, h, dt), wb, acc[dt]);
+    }
+  };
+  uint32_t bad = 0;   // a masked subtile held a non-finite value: the wave's rows are redone at the end
+  auto check = [&](const char* Xt) __attribute__((always_inline)) {
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) bad |= nonfinite(lds8(Xt, offK[kk]));
+  };
+  // a tile that every row of the wave sees whole: straight-line code, so the LDS reads of one
+  // subtile run under the softmax of its neighbour
+  auto body_full = [&](const char* Kt, const char* Vt) __attribute__((always_inline)) {
+    f32x16 s[NSUB];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < NSUB; ++t) s[t] = scores(Kt + 32 * t * RB);
+#pragma unroll
+    for (int t = 0; t < NSUB; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
+    const float mc = raise_max(mx);
+#pragma unroll
+    for (int t = 0; t < NSUB; ++t) expo(s[t], mc);
+#pragma unroll
+    for (int t = 0; t < NSUB; ++t) accum(Vt + 32 * t * RB, s[t]);
+  };
+  // a tile with skipped or masked subtiles, one subtile at a time
+  auto body_part = [&](const char* Kt, const char* Vt, int kt0) __attribute__((always_inline)) {
+    const int ta = max(0, (smin - kt0) >> 5), tb = min(NSUB - 1, (wlast - kt0) >> 5);
+#pragma unroll 1
+    for (int t = ta; t <= tb; ++t) {
+      const int k0 = kt0 + 32 * t;
+      const char *Ks = Kt + 32 * t * RB, *Vs = Vt + 32 * t * RB;
+      const bool masked = uni(k0 < smax || k0 + 31 > qw || qw + 31 >= nv ? 1 : 0);
+      f32x16 s = scores(Ks);
+      if constexpr (!DQ) {
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[e] = seen(k0, e) ? s[e] : -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[e]);
+        const float mc = raise_max(mx);
+        expo(s, mc);
+        if (masked) check(Vs);
+        accum(Vs, s);
+      } else {
+        f32x16 dp = f32x16{};
+#pragma unroll
+        for (int kk = 0; kk < NKK; ++kk) dp = mfma32(lds8(Vs, offK[kk]), dof[kk], dp);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -lse2)) * (dp[e] - dl);   // dS^T
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[e] = seen(k0, e) ? s[e] : 0.f;
+          check(Ks);
+        }
+        accum(Ks, s);
+      }
+    }
+  };
+  auto compute = [&](const char* Kt, const char* Vt, int j) __attribute__((always_inline)) {
+    const int k0 = kv_lo + j * BK;
+    if (uni(!wave_on || k0 > wlast || k0 + BK <= smin ? 1 : 0)) return;
+    if constexpr (!DQ) {
+      if (uni(k0 >= smax && k0 + BK <= qw + 1 && qw + 31 < nv ? 1 : 0)) {
+        body_full(Kt, Vt);
+        return;
+      }
+    }
+    body_part(Kt, Vt, k0);
+  };
+  auto step = [&](char* Kc, char* Vc, char* Kn, char* Vn, int j) __attribute__((always_inline)) {
+    vm_drain();
+    __syncthreads();
+    if (j + 1 < ntile) issue(Kn, Vn, j + 1);
+    compute(Kc, Vc, j);
+  };
+  issue(kbuf0, vbuf0, 0);
+  for (int j = 0; j < ntile; j += 2) {
+    step(kbuf0, vbuf0, kbuf1, vbuf1, j);
+    if (j + 1 < ntile) step(kbuf1, vbuf1, kbuf0, vbuf0, j + 1);
+  }
+
+  if (a.fill && qrow >= nv && qrow < T) {
+    zero_row<D>(outp, hh);
+    if (!DQ && hh == 0) a.lse[(size_t)hq * T + qrow] = INFINITY;
+  }
+  if (__any(bad != 0)) {
+#pragma unroll 1
+    for (int i = qw; i <= wlast; ++i) {
+      const RowVec<D> qi(a.q + (size_t)i * a.ldq + hq * D, lane);
+      RowVec<D> res;
+      float m = -INFINITY, l = 0.f, de = 0.f, ls = 0.f;
+      RowVec<D> doi;
+      if constexpr (DQ) {
+        doi = RowVec<D>(a.dout + (size_t)i * a.lddo + hq * D, lane);
+        de = doi.dot(RowVec<D>(a.o + (size_t)i * a.ldo + hq * D, lane));
+        ls = a.lse[(size_t)hq * T + i];
+      }
+#pragma unroll 1
+      for (int j = a.start[i]; j <= i; ++j) {
+        const RowVec<D> kj(a.k + (size_t)j * a.ldk + hk * D, lane);
+        const RowVec<D> vj(a.v + (size_t)j * a.ldv + hk * D, lane);
+        const float sij = qi.dot(kj);
+        if constexpr (!DQ) {
+          const float m_new = fmaxf(m, sij), mc = m_new == -INFINITY ? 0.f : m_new * c;
+          const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+          const float pij = __builtin_amdgcn_exp2f(__builtin_fmaf(sij, c, -mc));
+          m = m_new;
+          l = l * alpha + pij;
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x) res.x[x] *= alpha;
+          res.axpy(pij, vj);
+        } else {
+          res.axpy(__builtin_amdgcn_exp2f(__builtin_fmaf(sij, c, -ls)) * (doi.dot(vj) - de), kj);
+        }
+      }
+      const float nan = __uint_as_float(0x7fc00000u);
+      res.store(a.out + (size_t)i * a.ldout + hq * D, lane, DQ ? a.scale : l > 0.f ? 1.f / l : nan);
+      if (!DQ && lane == 0) a.lse[(size_t)hq * T + i] = l > 0.f ? m * c + __log2f(l) : nan;
+    }
+    return;
+  }
+  if (qrow >= nv) return;
+  float sc = a.scale;
+  if constexpr (!DQ) {
+    const float lt = xhalf_sum(l_i);
+    // lt = 0 only where every visible score is -inf: NaN, as the definition has it
+    sc = lt > 0.f ? 1.f / lt : __uint_as_float(0x7fc00000u);
+    if (hh == 0) a.lse[(size_t)hq * T + qrow] = lt > 0.f ? m_i * c + __log2f(lt) : sc;
+  }
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) store_row32(outp + 32 * dt, acc[dt], sc, hh);
+}
+
+// ============================================================================ key-major
+// dK, dV.  Four waves of 32 keys, key on the MFMA lane; Q / dO tiles of QT rows (and their lse,
+// delta) stream through a two-slot LDS-DMA ring, over the query heads of the key head's group.
+template <int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1))) void
+packed_kmajor_kernel(const PArgs a) {
+  constexpr int KB = 128, QT = 64, NQS = QT / 32, NKK = D / 16, NDT = D / 32;
+  constexpr int RB = D * 2, CPR = D / 8, RPP = 64 / CPR, TILE = QT * RB, PPW = TILE / 1024 / 4;
+  __shared__ __attribute__((aligned(16))) char qb0[TILE];
+  __shared__ __attribute__((aligned(16))) char qb1[TILE];
+  __shared__ __attribute__((aligned(16))) char ob0[TILE];
+  __shared__ __attribute__((aligned(16))) char ob1[TILE];
+  __shared__ __attribute__((aligned(16))) float lb0[64];
+  __shared__ __attribute__((aligned(16))) float lb1[64];
+  __shared__ __attribute__((aligned(16))) float db0[64];
+  __shared__ __attribute__((aligned(16))) float db1[64];
+  const int tid = threadIdx.x, lane = tid & 63, wl = uni(tid >> 6);
+  const int r = lane & 31, hh = lane >> 5, g = lane >> 4, gi = lane & 15;
+  const int T = a.T, nv = uni(a.meta[0]);
+  int rank, hk;
+  block_map(a.Hkv, rank, hk);
+  const int grp = a.Hq / a.Hkv;
+  const int k0 = rank * KB;                          // early blocks (most rows of a long sequence) first
+  const int kw = k0 + 32 * wl, key = kw + r;
+  uint16_t* dkp = a.dk + (size_t)key * a.lddk + hk * D;
+  uint16_t* dvp = a.dv + (size_t)key * a.lddv + hk * D;
+  if (k0 >= nv) {
+    if (a.fill && key < T) {
+      zero_row<D>(dkp, hh);
+      zero_row<D>(dvp, hh);
+    }
+    return;
+  }
+  const int qend = uni(a.end[min(k0 + KB, nv) - 1]);   // queries of the block: k0 .. qend - 1
+  const int nqt = (qend - k0 + QT - 1) / QT, items = nqt * grp;
+  const bool wave_on = kw < nv;
+  const int emin = uni(a.end[min(kw, nv - 1)]), emax = uni(a.end[min(kw + 31, nv - 1)]);
+  const int key_c = min(key, nv - 1);
+  const int cnt = key < nv ? a.end[key_c] - key : 0;   // rows that see this key: key .. key + cnt - 1
+  bf16x8 kf[NKK], vf[NKK];
+  {
+    const uint16_t* kp = a.k + (size_t)key_c * a.ldk + hk * D + 8 * hh;
+    const uint16_t* vp = a.v + (size_t)key_c * a.ldv + hk * D + 8 * hh;
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) {
+      kf[kk] = ld8(kp + 16 * kk);
+      vf[kk] = ld8(vp + 16 * kk);
+    }
+  }
+  f32x16 dvacc[NDT], dkacc[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) { dvacc[dt] = f32x16{}; dkacc[dt] = f32x16{}; }
+  __builtin_amdgcn_s_waitcnt(0);   // (see packed_qmajor_kernel)
+
+  int offQ[NKK];
+#pragma unroll
+  for (int kk = 0; kk < NKK; ++kk) offQ[kk] = toff<D>(r, 2 * kk + hh);
+  int offT[NDT][2];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) {
+    const int col = 32 * dt + 16 * (g & 1) + 4 * (gi & 3), row0 = 4 * hh + (gi >> 2);
+    offT[dt][0] = toff<D>(row0, col >> 3) + (col & 7) * 2;
+    offT[dt][1] = toff<D>(row0 + 8, col >> 3) + (col & 7) * 2;
+  }
+  uint32_t voQ[PPW], voO[PPW];
+#pragma unroll
+  for (int i = 0; i < PPW; ++i) {
+    const int R = (wl + 4 * i) * RPP + lane / CPR, ch = (lane % CPR) ^ swz<D>(R);
+    voQ[i] = (uint32_t)(R * a.ldq + ch * 8) * 2u;
+    voO[i] = (uint32_t)(R * a.lddo + ch * 8) * 2u;
+  }
+  auto issue = [&](char* qd, char* od, float* ld, float* dd, int hq, int qs) __attribute__((always_inline)) {
+    const int rows = min(QT, nv - qs);
+    const i32x4_t qr = rows_rsrc<D>(a.q + (size_t)qs * a.ldq + hq * D, rows, a.ldq);
+    const i32x4_t dr = rows_rsrc<D>(a.dout + (size_t)qs * a.lddo + hq * D, rows, a.lddo);
+#pragma unroll
+    for (int i = 0; i < PPW; ++i) {
+      dma16_buf(qr, voQ[i], qd + (wl + 4 * i) * 1024);
+      dma16_buf(dr, voO[i], od + (wl + 4 * i) * 1024);
+    }
+    if (wl < 2) {
+      const size_t li = (size_t)hq * T + min(qs + lane, nv - 1);
+      if (wl == 0) dma4(a.lse + li, (char*)ld);
+      else dma4(a.delta + li, (char*)dd);
+    }
+  };
+  const float c = a.c;
+  uint32_t bad = 0;   // (see packed_qmajor_kernel)
+  auto body = [&](const char* Qt, const char* Ot, const float* Lt, const float* Dt, int qs) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int u = 0; u < NQS; ++u) {
+      const int qsu = qs + 32 * u;
+      if (uni(qsu + 31 < kw || qsu >= emax ? 1 : 0)) continue;
+      f32x16 s = f32x16{}, dp = f32x16{};
+      const char* Qu = Qt + 32 * u * RB;
+      const char* Ou = Ot + 32 * u * RB;
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk) {
+        s = mfma32(lds8(Qu, offQ[kk]), kf[kk], s);
+        dp = mfma32(lds8(Ou, offQ[kk]), vf[kk], dp);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const float4 ls = *reinterpret_cast<const float4*>(Lt + 32 * u + 8 * (e >> 2) + 4 * hh);
+        const float4 de = *reinterpret_cast<const float4*>(Dt + 32 * u + 8 * (e >> 2) + 4 * hh);
+        s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -ls.x));
+        s[e + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], c, -ls.y));
+        s[e + 2] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 2], c, -ls.z));
+        s[e + 3] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 3], c, -ls.w));
+        dp[e] = s[e] * (dp[e] - de.x);
+        dp[e + 1] = s[e + 1] * (dp[e + 1] - de.y);
+        dp[e + 2] = s[e + 2] * (dp[e + 2] - de.z);
+        dp[e + 3] = s[e + 3] * (dp[e + 3] - de.w);
+      }
+      // whole: every row of the subtile sees every key of the wave
+      if (uni(qsu < kw + 31 || qsu + 32 > emin || kw + 31 >= nv ? 1 : 0)) {
+        asm volatile("" ::: "memory");   // a real branch
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const bool seen = (uint32_t)(qsu + 4 * hh - key + crow(e, 0)) < (uint32_t)cnt;
+          s[e] = seen ? s[e] : 0.f;
+          dp[e] = seen ? dp[e] : 0.f;
+        }
+#pragma unroll
+        for (int kk = 0; kk < NKK; ++kk) bad |= nonfinite(lds8(Qu, offQ[kk])) | nonfinite(lds8(Ou, offQ[kk]));
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bf16x8 pb = pack8(s, 8 * h);
+        const bf16x8 sb = pack8(dp, 8 * h);
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) {
+          const int ro = 16 * h * RB;
+          dvacc[dt] = mfma32(cat(tr_read(Ou + ro, offT[dt][0]), tr_read(Ou + ro, offT[dt][1])), pb, dvacc[dt]);
+          dkacc[dt] = mfma32(cat(tr_read(Qu + ro, offT[dt][0]), tr_read(Qu + ro, offT[dt][1])), sb, dkacc[dt]);
+        }
+      }
+    }
+  };
+  int hq_n = hk * grp, qs_n = k0;      // the item to fetch next
+  int qs_c = k0;
+  auto advance = [&]() __attribute__((always_inline)) {
+    qs_n += QT;
+    if (qs_n >= qend) { qs_n = k0; ++hq_n; }
+  };
+  auto step = [&](char* Qc, char* Oc, float* Lc, float* Dc, char* Qn, char* On, float* Ln, float* Dn,
+                  int t) __attribute__((always_inline)) {
+    vm_drain();
+    __syncthreads();
+    const int qs = qs_c;
+    if (t + 1 < items) {
+      issue(Qn, On, Ln, Dn, hq_n, qs_n);
+      qs_c = qs_n;
+      advance();
+    }
+    if (uni(wave_on && qs < emax && qs + QT > kw ? 1 : 0)) body(Qc, Oc, Lc, Dc, qs);
+  };
+  issue(qb0, ob0, lb0, db0, hq_n, qs_n);
+  advance();
+  for (int t = 0; t < items; t += 2) {
+    step(qb0, ob0, lb0, db0, qb1, ob1, lb1, db1, t);
+    if (t + 1 < items) step(qb1, ob1, lb1, db1, qb0, ob0, lb0, db0, t + 1);
+  }
+  if (a.fill && key >= nv && key < T) {
+    zero_row<D>(dkp, hh);
+    zero_row<D>(dvp, hh);
+  }
+  if (__any(bad != 0)) {
+#pragma unroll 1
+    for (int j = kw; j <= min(kw + 31, nv - 1); ++j) {
+      const RowVec<D> kj(a.k + (size_t)j * a.ldk + hk * D, lane);
+      const RowVec<D> vj(a.v + (size_t)j * a.ldv + hk * D, lane);
+      RowVec<D> rk, rv;
+      const int je = a.end[j];
+#pragma unroll 1
+      for (int hq = hk * grp; hq < hk * grp + grp; ++hq)
+#pragma unroll 1
+        for (int i = j; i < je; ++i) {
+          const RowVec<D> qi(a.q + (size_t)i * a.ldq + hq * D, lane);
+          const RowVec<D> doi(a.dout + (size_t)i * a.lddo + hq * D, lane);
+          const size_t li = (size_t)hq * T + i;
+          const float pij = __builtin_amdgcn_exp2f(__builtin_fmaf(qi.dot(kj), c, -a.lse[li]));
+          rv.axpy(pij, doi);
+          rk.axpy(pij * (doi.dot(vj) - a.delta[li]), qi);
+        }
+      rk.store(a.dk + (size_t)j * a.lddk + hk * D, lane, a.scale);
+      rv.store(a.dv + (size_t)j * a.lddv + hk * D, lane, 1.f);
+    }
+    return;
+  }
+  if (key >= nv) return;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) {
+    store_row32(dkp + 32 * dt, dkacc[dt], a.scale, hh);
+    store_row32(dvp + 32 * dt, dvacc[dt], 1.f, hh);
+  }
+}
+
+bool bad_mat(const void* p, int ld, int width) {   // 16-B rows, tile offsets below 2^31 bytes
+  return p == nullptr || ((uintptr_t)p & 15) || (ld & 7) || ld < width || ld > (1 << 22);
+}
+bool bad_shape(int T, int Hq, int Hkv, int D) {
+  if (T <= 0 || T > (1 << 30) || Hq <= 0 || Hkv <= 0 || Hq % Hkv || (D != 64 && D != 128)) return true;
+  return (int64_t)((T + 127) / 128) * Hq >= ((int64_t)1 << 31);
+}
+
+}  // namespace
+
+// Row table of a packed batch (packed_plan_kernel).  cu: n + 1 cumulative lengths (int64 when
+// `wide`, else int32); start, end: int32 [T]; meta: int32 [4]; pos: int64 [T].
+MX_EXPORT int mx_packed_plan(const void* cu, int wide, int n, int T, int* start, int* end, int* meta, void* pos,
+                             hipStream_t s) {
+  if (!cu || !start || !end || !meta || !pos || n < 1 || T <= 0 || T > (1 << 30)) return hipErrorInvalidValue;
+  const dim3 grid((T + 255) / 256);
+  if (wide)
+    hipLaunchKernelGGL((packed_plan_kernel<int64_t>), grid, dim3(256), 0, s, (const int64_t*)cu, n, T, start, end,
+                       meta, (int64_t*)pos);
+  else
+    hipLaunchKernelGGL((packed_plan_kernel<int32_t>), grid, dim3(256), 0, s, (const int32_t*)cu, n, T, start, end,
+                       meta, (int64_t*)pos);
+  return hipGetLastError();
+}
+
+// Q, K, V, O: bf16 [T] rows with strides ld*, head h at column h D.  lse: fp32 [Hq][T], base 2.
+// fill: rows behind the last sequence get o = 0, lse = +inf; else they are left as they are.
+MX_EXPORT int mx_packed_attn_fwd(const void* q, const void* k, const void* v, int ldq, int ldk, int ldv, void* o,
+                                 int ldo, float* lse, const int* start, const int* end, const int* meta, int T,
+                                 int Hq, int Hkv, int D, float scale, int fill, hipStream_t s) {
+  if (bad_shape(T, Hq, Hkv, D) || bad_mat(q, ldq, Hq * D) || bad_mat(k, ldk, Hkv * D) || bad_mat(v, ldv, Hkv * D) ||
+      bad_mat(o, ldo, Hq * D) || !lse || !start || !end || !meta || !(scale > 0.f))
+    return hipErrorInvalidValue;
+  PArgs a{};
+  a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
+  a.out = (uint16_t*)o;
+  a.lse = lse;
+  a.start = start; a.end = end; a.meta = meta;
+  a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldout = ldo;
+  a.T = T; a.Hq = Hq; a.Hkv = Hkv;
+  a.c = scale * 1.4426950408889634f;
+  a.scale = scale;
+  a.fill = fill;
+  const dim3 grid((unsigned)((T + 127) / 128 * Hq));
+  if (D == 64) hipLaunchKernelGGL((packed_qmajor_kernel<64, false>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((packed_qmajor_kernel<128, false>), grid, dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+// delta: fp32 [Hq][T] workspace (written by the dQ kernel, read by the dK / dV kernel).
+MX_EXPORT int mx_packed_attn_bwd(const void* q, const void* k, const void* v, int ldq, int ldk, int ldv,
+                                 const void* o, int ldo, const void* dout, int lddo, const float* lse, float* delta,
+                                 void* dq, int lddq, void* dk, void* dv, int lddk, int lddv, const int* start,
+                                 const int* end, const int* meta, int T, int Hq, int Hkv, int D, float scale,
+                                 int fill, hipStream_t s) {
+  if (bad_shape(T, Hq, Hkv, D) || bad_mat(q, ldq, Hq * D) || bad_mat(k, ldk, Hkv * D) || bad_mat(v, ldv, Hkv * D) ||
+      bad_mat(o, ldo, Hq * D) || bad_mat(dout, lddo, Hq * D) || bad_mat(dq, lddq, Hq * D) ||
+      bad_mat(dk, lddk, Hkv * D) || bad_mat(dv, lddv, Hkv * D) || !lse || !delta || !start || !end || !meta ||
+      !(scale > 0.f))
+    return hipErrorInvalidValue;
+  PArgs a{};
+  a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
+  a.o = (const uint16_t*)o; a.dout = (const uint16_t*)dout;
+  a.out = (uint16_t*)dq; a.dk = (uint16_t*)dk; a.dv = (uint16_t*)dv;
+  a.lse = const_cast<float*>(lse);
+  a.delta = delta;
+  a.start = start; a.end = end; a.meta = meta;
+  a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo; a.lddo = lddo; a.ldout = lddq; a.lddk = lddk; a.lddv = lddv;
+  a.T = T; a.Hq = Hq; a.Hkv = Hkv;
+  a.c = scale * 1.4426950408889634f;
+  a.scale = scale;
+  a.fill = fill;
+  const unsigned nb = (unsigned)((T + 127) / 128);
+  if (D == 64) {
+    hipLaunchKernelGGL((packed_qmajor_kernel<64, true>), dim3(nb * Hq), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((packed_kmajor_kernel<64>), dim3(nb * Hkv), dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((packed_qmajor_kernel<128, true>), dim3(nb * Hq), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((packed_kmajor_kernel<128>), dim3(nb * Hkv), dim3(256), 0, s, a);
+  }
+  return hipGetLastError();
+}

@@ -112,6 +112,10 @@ SIGNATURES = {
     "mx_gemm_nt_tile": [I, I],
     "mx_gemm_nt": [P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, P],
     "mx_gemm_nt_stamps": [P, P, P, P, I, I, I, I, I, I, I, P],
+    # packed.hip
+    "mx_packed_plan": [P, I, I, I, P, P, P, P, P],
+    "mx_packed_attn_fwd": [P, P, P, I, I, I, P, I, P, P, P, P, I, I, I, I, F, I, P],
+    "mx_packed_attn_bwd": [P, P, P, I, I, I, P, I, P, I, P, P, P, I, P, P, I, I, P, P, P, I, I, I, I, F, I, P],
     # rope.hip
     "mx_rope": [P, I64, I, I, I, I, I, I, I, P, P, P, I, P],
     # vision.hip

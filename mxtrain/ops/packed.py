@@ -1,0 +1,245 @@
+"""Packed causal attention (``csrc/packed.hip``) + reference: sequences of different lengths laid
+end to end on one token axis, grouped heads, no attention across a border.
+
+:func:`pack_sequences` builds the row table of a batch from its cumulative lengths -- once per
+batch, shared by every layer and by forward and backward.  Tensors are token-major 2-D views
+[T, H * D] with any row stride (the packed QKV projection output is read in place), as in
+``ops/attention.py``; ``lse`` is the base-2 log-sum-exp [Hq, T] the backward needs.
+
+Rows behind the last sequence (a batch padded to a fixed size, so a captured step keeps its
+shapes) are never read: in tensors the op allocates they are zero, in buffers the caller passes
+they are left as they were.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+LOG2E = 1.4426950408889634
+
+
+class PackedSequences:
+    """Row table of one packed batch: ``cu_seqlens`` [n + 1] and, for each of ``total`` rows,
+    the bounds of its sequence (``start``, ``end``, int32) and its position in it
+    (``positions``, int64: RoPE's ``pos_ids``, the rows of a learned position table)."""
+
+    __slots__ = ("cu_seqlens", "total", "start", "end", "meta", "positions")
+
+    def __init__(self, cu_seqlens, total, start, end, meta, positions):
+        self.cu_seqlens, self.total = cu_seqlens, total
+        self.start, self.end, self.meta, self.positions = start, end, meta, positions
+
+    @property
+    def device(self):
+        return self.start.device
+
+
+def pack_sequences(cu_seqlens: torch.Tensor, total: int, device=None) -> PackedSequences:
+    """``cu_seqlens``: [n + 1] int32 / int64 cumulative lengths, first 0, non-decreasing, last
+    <= ``total`` (the rows of the batch; the rows behind the last sequence belong to none).
+    A sequence may have length zero.  A CPU tensor is checked; a tensor on the GPU is not (that
+    would wait for the device): its values are clamped into range by the kernel, so a table
+    that breaks the contract gives wrong sequences, not an access out of range."""
+    if cu_seqlens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"pack_sequences: cu_seqlens must be int32 or int64, got {cu_seqlens.dtype}")
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
+        raise ValueError("pack_sequences: cu_seqlens must be a 1-D tensor of at least two entries")
+    total = int(total)
+    if not 0 < total <= 1 << 30:
+        raise ValueError(f"pack_sequences: total must be in 1 .. 2^30, got {total}")
+    if not cu_seqlens.is_cuda:
+        c = cu_seqlens.tolist()
+        if c[0] != 0 or c[-1] > total or any(b < a for a, b in zip(c, c[1:])):
+            raise ValueError(f"pack_sequences: cu_seqlens must start at 0, not decrease and end at most at {total}")
+    dev = torch.device(device) if device is not None else cu_seqlens.device
+    cu = cu_seqlens.to(dev).contiguous()
+    n = cu.numel() - 1
+    if not _lib.use_hip(cu):
+        t = torch.arange(total, device=dev)
+        nv = int(cu[-1])
+        i = (torch.searchsorted(cu.to(torch.int64), t, right=True) - 1).clamp_(0, n - 1)
+        real = t < nv
+        start = torch.where(real, cu.to(torch.int64)[i], t)
+        end = torch.where(real, cu.to(torch.int64)[i + 1], t)
+        meta = torch.tensor([nv, 0, 0, 0], dtype=torch.int32, device=dev)
+        return PackedSequences(cu, total, start.int(), end.int(), meta, t - start)
+    with torch.cuda.device(cu.device):
+        tab = torch.empty(2 * total + 4, dtype=torch.int32, device=cu.device)
+        pos = torch.empty(total, dtype=torch.int64, device=cu.device)
+        start, end, meta = tab[:total], tab[total:2 * total], tab[2 * total:]
+        _lib.call("mx_packed_plan", _lib.ptr(cu), int(cu.dtype == torch.int64), n, total, _lib.ptr(start),
+                  _lib.ptr(end), _lib.ptr(meta), _lib.ptr(pos), _lib.stream())
+    return PackedSequences(cu, total, start, end, meta, pos)
+
+
+# ------------------------------------------------------------------ checks
+def _check(name, seqs, Hq, Hkv, D, scale, **mats):
+    if not isinstance(seqs, PackedSequences):
+        raise TypeError(f"{name}: seqs must come from pack_sequences()")
+    if Hq <= 0 or Hkv <= 0 or Hq % Hkv:
+        raise ValueError(f"{name}: Hq ({Hq}) must be a positive multiple of Hkv ({Hkv})")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"{name}: scale must be positive and finite, got {scale}")
+    q = mats["q"]
+    hip = _lib.use_hip(q)
+    if hip and D not in (64, 128):
+        raise ValueError(f"{name}: the GPU kernels take a head dimension of 64 or 128, got {D}")
+    for key, t in mats.items():
+        if t is None:
+            continue
+        width = (Hkv if key in ("k", "v", "dk", "dv") else Hq) * D
+        if t.dim() != 2 or t.shape[0] != seqs.total or t.shape[1] != width:
+            raise ValueError(f"{name}: {key} must be [{seqs.total}, {width}], got {list(t.shape)}")
+        if t.device != seqs.device:
+            raise ValueError(f"{name}: {key} is on {t.device}, the sequences on {seqs.device}")
+        if t.dtype != q.dtype:
+            raise TypeError(f"{name}: {key} is {t.dtype}, q is {q.dtype}")
+        if hip:
+            if t.dtype != torch.bfloat16:
+                raise TypeError(f"{name}: the GPU kernels take bfloat16, {key} is {t.dtype}")
+            if not _readable(t) or _ld(t) > 1 << 22:
+                raise ValueError(f"{name}: {key} needs unit column stride, rows that do not overlap, a row stride "
+                                 f"that is a multiple of 8 (at most 2^22) and 16-byte alignment; strides "
+                                 f"{list(t.stride())}, address % 16 = {t.data_ptr() % 16}")
+    return scale, hip
+
+
+def _ld(t):
+    """Row stride (a single row has none: its width)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _readable(t):
+    """Rows the kernels read (and write) in place."""
+    return (t.dim() == 2 and t.stride(1) == 1 and _ld(t) % 8 == 0 and _ld(t) >= t.shape[1]
+            and t.data_ptr() % 16 == 0)
+
+
+def _check_lse(name, lse, Hq, seqs):
+    if tuple(lse.shape) != (Hq, seqs.total) or lse.dtype != torch.float32 or not lse.is_contiguous() \
+            or lse.device != seqs.device:
+        raise ValueError(f"{name}: lse must be the float32 [{Hq}, {seqs.total}] tensor packed_attn_fwd returned")
+
+
+# ------------------------------------------------------------------ reference (CPU)
+def _ref_mask(seqs):
+    t = torch.arange(seqs.total, device=seqs.device)
+    real = (t < seqs.meta[0])[:, None]
+    return real & (t[None, :] <= t[:, None]) & (t[None, :] >= seqs.start[:, None])
+
+
+def _acc(t):   # at least float32
+    return t.double() if t.dtype == torch.float64 else t.float()
+
+
+def _ref_fwd(q, k, v, seqs, Hq, Hkv, D, scale):
+    T = seqs.total
+    real = torch.arange(T, device=q.device) < seqs.meta[0]
+
+    def heads(t, h):   # [h, T, D]; the rows behind the last sequence are never read
+        return torch.where(real[:, None], _acc(t), torch.zeros((), dtype=_acc(t).dtype)).reshape(T, h, D).transpose(0, 1)
+    g = Hq // Hkv
+    qf, kf, vf = heads(q, Hq), heads(k, Hkv).repeat_interleave(g, 0), heads(v, Hkv).repeat_interleave(g, 0)
+    m = _ref_mask(seqs)
+    s = (torch.matmul(qf, kf.transpose(1, 2)) * scale).masked_fill(~m, float("-inf"))
+    lse = torch.logsumexp(s, -1)
+    p = torch.where(m, torch.exp(s - lse[..., None]), torch.zeros((), dtype=s.dtype))
+    o = torch.matmul(p, vf).transpose(0, 1).reshape(T, Hq * D)
+    lse = torch.where(real, lse * LOG2E, torch.full_like(lse, float("inf")))
+    return o, lse
+
+
+def _emit(val, buf, seqs):
+    """``val`` rounded to the result: a new tensor (zero behind the last sequence), or into the
+    caller's buffer, whose rows there stay as they are."""
+    if buf is None:
+        return val
+    nv = int(seqs.meta[0])
+    buf[:nv] = val[:nv].to(buf.dtype)
+    return buf
+
+
+# ------------------------------------------------------------------ forward / backward
+def packed_attn_fwd(q, k, v, seqs: PackedSequences, Hq: int, Hkv: int, D: int, scale: Optional[float] = None,
+                    out=None):
+    """Causal attention within each sequence: q [T, Hq*D], k / v [T, Hkv*D] -> (o [T, Hq*D],
+    lse [Hq, T]).  Query head h reads key head h // (Hq // Hkv).  ``out``: a buffer for o."""
+    scale, hip = _check("packed_attn_fwd", seqs, Hq, Hkv, D, scale, q=q, k=k, v=v, out=out)
+    if not hip:
+        o, lse = _ref_fwd(q, k, v, seqs, Hq, Hkv, D, scale)
+        return _emit(o.to(q.dtype), out, seqs), lse.float()
+    with torch.cuda.device(q.device):
+        o = out if out is not None else torch.empty(seqs.total, Hq * D, dtype=q.dtype, device=q.device)
+        lse = torch.empty(Hq, seqs.total, dtype=torch.float32, device=q.device)
+        _lib.call("mx_packed_attn_fwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _ld(q), _ld(k), _ld(v),
+                  _lib.ptr(o), _ld(o), _lib.ptr(lse), _lib.ptr(seqs.start), _lib.ptr(seqs.end),
+                  _lib.ptr(seqs.meta), seqs.total, Hq, Hkv, D, scale, int(out is None), _lib.stream())
+    return o, lse
+
+
+def packed_attn_bwd(dout, q, k, v, o, lse, seqs: PackedSequences, Hq: int, Hkv: int, D: int,
+                    scale: Optional[float] = None, dq=None, dk=None, dv=None):
+    """(dq, dk, dv) of :func:`packed_attn_fwd`; given views (e.g. column ranges of one packed
+    dqkv) are written in place.  Deterministic: no atomics."""
+    scale, hip = _check("packed_attn_bwd", seqs, Hq, Hkv, D, scale, q=q, k=k, v=v, dout=dout, o=o, dq=dq, dk=dk,
+                        dv=dv)
+    _check_lse("packed_attn_bwd", lse, Hq, seqs)
+    if not hip:
+        with torch.enable_grad():
+            leaves = [_acc(t.detach()).clone().requires_grad_(True) for t in (q, k, v)]
+            of, _ = _ref_fwd(*leaves, seqs, Hq, Hkv, D, scale)
+            nv = int(seqs.meta[0])
+            grads = torch.autograd.grad(of[:nv], leaves, _acc(dout)[:nv])
+        return tuple(_emit(g.to(q.dtype), buf, seqs) for g, buf in zip(grads, (dq, dk, dv)))
+    given = [t is not None for t in (dq, dk, dv)]
+    if any(given) and not all(given):
+        raise ValueError("packed_attn_bwd: give all of dq, dk, dv or none")
+    if given[0] and {t.data_ptr() for t in (dq, dk, dv)} & {t.data_ptr() for t in (q, k, v, o, dout)}:
+        raise ValueError("packed_attn_bwd: dq, dk, dv must not lie over q, k, v, o or dout (read after they are written)")
+    with torch.cuda.device(q.device):
+        if dq is None:
+            dq = torch.empty(seqs.total, Hq * D, dtype=q.dtype, device=q.device)
+            dk = torch.empty(seqs.total, Hkv * D, dtype=q.dtype, device=q.device)
+            dv = torch.empty(seqs.total, Hkv * D, dtype=q.dtype, device=q.device)
+        delta = torch.empty(Hq, seqs.total, dtype=torch.float32, device=q.device)
+        _lib.call("mx_packed_attn_bwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _ld(q), _ld(k), _ld(v),
+                  _lib.ptr(o), _ld(o), _lib.ptr(dout), _ld(dout), _lib.ptr(lse), _lib.ptr(delta),
+                  _lib.ptr(dq), _ld(dq), _lib.ptr(dk), _lib.ptr(dv), _ld(dk), _ld(dv),
+                  _lib.ptr(seqs.start), _lib.ptr(seqs.end), _lib.ptr(seqs.meta), seqs.total, Hq, Hkv, D, scale,
+                  int(not given[0]), _lib.stream())
+    return dq, dk, dv
+
+
+class PackedAttnFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, seqs, Hq, Hkv, D, scale):
+        q, k, v = (_rows(t) for t in (q, k, v))
+        o, lse = packed_attn_fwd(q, k, v, seqs, Hq, Hkv, D, scale)
+        ctx.save_for_backward(q, k, v, o, lse)
+        ctx.meta = (seqs, Hq, Hkv, D, scale)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse = ctx.saved_tensors
+        seqs, Hq, Hkv, D, scale = ctx.meta
+        dq, dk, dv = packed_attn_bwd(_rows(do), q, k, v, o, lse, seqs, Hq, Hkv, D, scale)
+        return dq, dk, dv, None, None, None, None, None
+
+
+def _rows(t):
+    """``t`` itself when the kernels can read it in place, else a contiguous copy (an expanded
+    or transposed tensor, an unaligned view)."""
+    return t if not t.is_cuda or _readable(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def packed_attention(q, k, v, seqs: PackedSequences, Hq: int, Hkv: int, D: int, scale: Optional[float] = None):
+    """Differentiable packed causal attention (see :func:`packed_attn_fwd`).  First derivatives
+    only."""
+    return PackedAttnFn.apply(q, k, v, seqs, Hq, Hkv, D, scale)

@@ -1,0 +1,85 @@
+"""Packed attention on the CPU path: the row table, refusals, the formula and its gradients."""
+import pytest
+import torch
+
+from mxtrain import ops
+from packed_oracle import attention, within
+
+
+def _cu(lens):
+    return torch.tensor([0] + list(lens)).cumsum(0)
+
+
+def test_row_table():
+    s = ops.pack_sequences(_cu([3, 0, 0, 1, 4]), 10)
+    assert s.start.tolist() == [0, 0, 0, 3, 4, 4, 4, 4, 8, 9]
+    assert s.end.tolist() == [3, 3, 3, 4, 8, 8, 8, 8, 8, 9]
+    assert s.positions.tolist() == [0, 1, 2, 0, 0, 1, 2, 3, 0, 0]
+    assert int(s.meta[0]) == 8
+
+
+def test_row_table_of_empty_sequences():
+    s = ops.pack_sequences(_cu([0, 0]).int(), 3)
+    assert int(s.meta[0]) == 0 and s.positions.tolist() == [0, 0, 0]
+
+
+@pytest.mark.parametrize("cu,total,err", [
+    (torch.tensor([0.0, 3.0]), 3, TypeError),
+    (torch.tensor([[0, 3]]), 3, ValueError),
+    (torch.tensor([0]), 3, ValueError),
+    (torch.tensor([1, 3]), 3, ValueError),
+    (torch.tensor([0, 3, 2]), 3, ValueError),
+    (torch.tensor([0, 4]), 3, ValueError),
+    (torch.tensor([0, 3]), 0, ValueError),
+])
+def test_row_table_refusals(cu, total, err):
+    with pytest.raises(err):
+        ops.pack_sequences(cu, total)
+
+
+def test_attention_refusals():
+    s = ops.pack_sequences(_cu([5, 3]), 8)
+    q, k = torch.randn(8, 4 * 16), torch.randn(8, 2 * 16)
+    for args, kw, err in (
+            ((q, k, k, s, 4, 3, 16), {}, ValueError),            # heads do not group
+            ((q[:7], k, k, s, 4, 2, 16), {}, ValueError),        # rows
+            ((q, k[:, :16], k, s, 4, 2, 16), {}, ValueError),    # width
+            ((q, k.double(), k, s, 4, 2, 16), {}, TypeError),    # types differ
+            ((q, k, k, s, 4, 2, 16, -1.0), {}, ValueError),      # scale
+            ((q, k, k, s, 4, 2, 16, float("nan")), {}, ValueError),
+            ((q, k, k, [0, 5, 8], 4, 2, 16), {}, TypeError),
+            ((q, k, k, s, 4, 2, 16), {"out": torch.empty(8, 16)}, ValueError)):
+        with pytest.raises(err):
+            ops.packed_attn_fwd(*args, **kw)
+    o, lse = ops.packed_attn_fwd(q, k, k, s, 4, 2, 16)
+    with pytest.raises(ValueError):
+        ops.packed_attn_bwd(o, q, k, k, o, lse[:, :4], s, 4, 2, 16)
+
+
+@pytest.mark.parametrize("lens,pad", [([1], 0), ([5, 0, 9, 1], 3), ([0], 2)])
+def test_reference_matches_oracle(lens, pad):
+    torch.manual_seed(1)
+    T, Hq, Hkv, D = sum(lens) + pad, 4, 2, 16
+    q, k, v, do = (torch.randn(T, h * D, dtype=torch.float64) for h in (Hq, Hkv, Hkv, Hq))
+    s = ops.pack_sequences(_cu(lens), T)
+    o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D)
+    dq, dk, dv = ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D)
+    want = attention(q, k, v, lens, Hq, Hkv, D, D ** -0.5, do)
+    for name, t in (("o", o), ("dq", dq), ("dk", dk), ("dv", dv)):
+        torch.testing.assert_close(t, want[name][0], rtol=1e-12, atol=1e-12)   # float64 on both sides
+        assert (t[sum(lens):] == 0).all()
+
+
+def test_gradients_against_differences():
+    torch.manual_seed(2)
+    s = ops.pack_sequences(_cu([4, 1, 3]), 9)
+    q, k, v = (torch.randn(9, h * 8, dtype=torch.float64, requires_grad=True) for h in (4, 2, 2))
+    assert torch.autograd.gradcheck(lambda a, b, c: ops.packed_attention(a, b, c, s, 4, 2, 8), (q, k, v))
+
+
+def test_buffers_keep_the_rows_behind():
+    s = ops.pack_sequences(_cu([2, 3]), 8)
+    q = torch.randn(8, 16)
+    out = torch.full((8, 16), 7.0)
+    ops.packed_attn_fwd(q, q, q, s, 1, 1, 16, out=out)
+    assert (out[5:] == 7.0).all() and not (out[:5] == 7.0).any()

@@ -1,0 +1,249 @@
+"""Packed attention kernels (csrc/packed.hip) against the 64-bit oracle and its derived bounds."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from mxtrain import ops  # noqa: E402
+from packed_oracle import attention, within  # noqa: E402
+
+DEV = "cuda"
+
+
+def _cu(lens):
+    return torch.tensor([0] + list(lens)).cumsum(0)
+
+
+def _inputs(T, Hq, Hkv, D, seed=0, gap=0):
+    """q, k, v as column ranges of one buffer (row stride wider than the heads by ``gap``)."""
+    gen = torch.Generator().manual_seed(seed)
+    buf = torch.randn(T, (Hq + 2 * Hkv) * D + gap, generator=gen).to(torch.bfloat16).to(DEV)
+    do = torch.randn(T, Hq * D, generator=gen).to(torch.bfloat16).to(DEV)
+    q, k, v = buf[:, :Hq * D], buf[:, Hq * D:(Hq + Hkv) * D], buf[:, (Hq + Hkv) * D:(Hq + 2 * Hkv) * D]
+    return q, k, v, do
+
+
+LENS = [
+    ([1], 0), ([1, 1, 1], 1), ([0, 5, 0], 0), ([31, 32, 33], 0), ([127, 1, 129], 3), ([128, 128], 0),
+    ([64, 2, 190, 0, 77], 51), ([300], 129), ([3] * 100, 0), ([513, 200], 0), ([0, 0], 4),
+]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("heads", [(2, 2), (8, 2), (3, 1)])
+@pytest.mark.parametrize("lens,pad", LENS)
+def test_forward_backward(lens, pad, heads, D):
+    Hq, Hkv = heads
+    T = sum(lens) + pad
+    q, k, v, do = _inputs(T, Hq, Hkv, D, seed=T, gap=8)
+    s = ops.pack_sequences(_cu(lens), T, device=DEV)
+    o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D)
+    dq, dk, dv = ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D)
+    want = attention(q, k, v, lens, Hq, Hkv, D, D ** -0.5, do)
+    for name, t in (("o", o), ("lse", lse), ("dq", dq), ("dk", dk), ("dv", dv)):
+        within(t, want[name], name)
+
+
+@pytest.mark.parametrize("D,lens,heads", [(64, [2500, 1, 700, 895], (4, 2)), (128, [1500, 2600], (2, 1))])
+def test_longer_sequences(D, lens, heads):
+    Hq, Hkv = heads
+    T = sum(lens) + 77
+    q, k, v, do = _inputs(T, Hq, Hkv, D, seed=5)
+    s = ops.pack_sequences(_cu(lens), T, device=DEV)
+    o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D, scale=0.3)
+    grads = ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D, scale=0.3)
+    want = attention(q, k, v, lens, Hq, Hkv, D, 0.3, do)
+    for name, t in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+        within(t, want[name], name)
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_row_table_matches_cpu(dtype):
+    lens = [0, 3, 0, 0, 260, 1, 77, 0]
+    cu = _cu(lens).to(dtype)
+    for given in (cu, cu.to(DEV)):
+        a, b = ops.pack_sequences(given, 400, device=DEV), ops.pack_sequences(cu, 400)
+        for f in ("start", "end", "positions"):
+            assert torch.equal(getattr(a, f).cpu(), getattr(b, f)), f
+        assert int(a.meta[0]) == int(b.meta[0])
+
+
+def test_malformed_table_on_the_gpu_stays_in_range():
+    cu = torch.tensor([5, -3, 900, 40, 1 << 40], device=DEV)
+    s = ops.pack_sequences(cu, 200)
+    t = torch.arange(200, device=DEV)
+    assert ((s.start >= 0) & (s.start <= t)).all() and ((s.end > t) & (s.end <= 200)).all()
+    assert int(s.meta[0]) == 200
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_non_finite_values_stay_in_their_sequence(D, bad):
+    """Sequences 0, 2 and the rows behind the end hold non-finite values; sequence 1 and 3 must
+    get exactly what they get beside finite neighbours."""
+    lens, pad, H = [40, 50, 70, 30], 20, 2
+    T = sum(lens) + pad
+    q, k, v, do = _inputs(T, H, H, D, seed=3)
+    s = ops.pack_sequences(_cu(lens), T, device=DEV)
+    clean = ops.packed_attn_fwd(q, k, v, s, H, H, D)
+    cleang = ops.packed_attn_bwd(do, q, k, v, *clean, s, H, H, D)
+    want = attention(q, k, v, lens, H, H, D, D ** -0.5, do)
+    for t in (q, k, v, do):
+        t[10:20] = bad
+        t[100:110] = bad
+        t[190:] = bad
+    o, lse = ops.packed_attn_fwd(q, k, v, s, H, H, D)
+    grads = ops.packed_attn_bwd(do, q, k, v, o, lse, s, H, H, D)
+    for name, t in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+        for rows in (slice(40, 90), slice(160, 190)):
+            within(t[rows], tuple(x[rows] for x in want[name]), name)
+        assert (t[190:] == 0).all(), name
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_later_rows_do_not_reach_earlier_ones(D):
+    """A NaN row inside a sequence: the rows before it see none of it; the rows from it on do."""
+    T, H, at = 200, 2, 75
+    q, k, v, do = _inputs(T, H, H, D, seed=4)
+    s = ops.pack_sequences(_cu([T]), T, device=DEV)
+    want = attention(q, k, v, [T], H, H, D, D ** -0.5)
+    v[at] = float("nan")
+    o, _ = ops.packed_attn_fwd(q, k, v, s, H, H, D)
+    within(o[:at], tuple(x[:at] for x in want["o"]), "o")
+    assert torch.isnan(o[at:]).all()
+    q, k, v, do = _inputs(T, H, H, D, seed=4)
+    o, lse = ops.packed_attn_fwd(q, k, v, s, H, H, D)
+    want = attention(q, k, v, [T], H, H, D, D ** -0.5, do)
+    do[at] = float("nan")      # row `at` touches the keys up to it alone
+    dq, dk, dv = ops.packed_attn_bwd(do, q, k, v, o, lse, s, H, H, D)
+    for name, t in (("dk", dk), ("dv", dv)):
+        within(t[at + 1:], tuple(x[at + 1:] for x in want[name]), name)
+        assert torch.isnan(t[:at + 1]).all()
+    keep = torch.arange(T, device=DEV) != at
+    within(dq[keep], tuple(x[keep] for x in want["dq"]), "dq")
+
+
+def test_extreme_scores():
+    """Rows whose scores span far more than the range of exp; the largest must win exactly."""
+    T, H, D = 150, 2, 64
+    q, k, v, _ = _inputs(T, H, H, D, seed=8)
+    q.mul_(64.0)
+    k.mul_(64.0)
+    s = ops.pack_sequences(_cu([T]), T, device=DEV)
+    o, _ = ops.packed_attn_fwd(q, k, v, s, H, H, D)
+    assert torch.isfinite(o).all()
+    top = torch.stack([(q[:, h * D:(h + 1) * D].double() @ k[:, h * D:(h + 1) * D].double().t())
+                       .masked_fill(torch.ones(T, T, dtype=torch.bool, device=DEV).triu(1), -1e300).argmax(1)
+                       for h in range(H)])
+    for h in range(H):
+        sc = (q[:, h * D:(h + 1) * D].double() @ k[:, h * D:(h + 1) * D].double().t()) * D ** -0.5
+        sc = sc.masked_fill(torch.ones(T, T, dtype=torch.bool, device=DEV).triu(1), -1e300)
+        two = sc.topk(2, 1).values if T > 1 else sc
+        clear = two[:, 0] - two[:, 1] > 40.0       # every other weight is below 2^-57
+        got = o[:, h * D:(h + 1) * D]
+        assert torch.equal(got[clear], v[top[h][clear], h * D:(h + 1) * D])
+
+
+def test_buffers_and_rows_behind():
+    lens, pad, Hq, Hkv, D = [100, 33], 60, 4, 2, 64
+    T = sum(lens) + pad
+    q, k, v, do = _inputs(T, Hq, Hkv, D, seed=6)
+    s = ops.pack_sequences(_cu(lens), T, device=DEV)
+    o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D)
+    assert (o[133:] == 0).all() and torch.isinf(lse[:, 133:]).all()
+    buf = torch.full((T, Hq * D + 64), 3.0, dtype=torch.bfloat16, device=DEV)
+    out, _ = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D, out=buf[:, 64:])
+    assert torch.equal(out[:133], o[:133]) and (buf[133:] == 3.0).all() and (buf[:, :64] == 3.0).all()
+    ref = ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D)
+    pack = torch.full((T, (Hq + 2 * Hkv) * D), 3.0, dtype=torch.bfloat16, device=DEV)
+    views = pack[:, :Hq * D], pack[:, Hq * D:(Hq + Hkv) * D], pack[:, (Hq + Hkv) * D:]
+    ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D, dq=views[0], dk=views[1], dv=views[2])
+    for a, b in zip(views, ref):
+        assert torch.equal(a[:133], b[:133]) and (b[133:] == 0).all()
+    assert (pack[133:] == 3.0).all()
+
+
+def test_refusals():
+    s = ops.pack_sequences(_cu([8]), 8, device=DEV)
+    q = torch.randn(8, 128, device=DEV, dtype=torch.bfloat16)
+    big = torch.randn(8, 136, device=DEV, dtype=torch.bfloat16)
+    for args, err in (((q.half(), q.half(), q.half(), s, 2, 2, 64), TypeError),
+                      ((q, q, q, s, 4, 4, 32), ValueError),                         # head dimension
+                      ((big[:, 1:129], q, q, s, 2, 2, 64), ValueError),             # alignment
+                      ((q[:1].expand(8, 128), q, q, s, 2, 2, 64), ValueError),      # rows that overlap
+                      ((q, q.cpu(), q, s, 2, 2, 64), ValueError)):
+        with pytest.raises(err):
+            ops.packed_attn_fwd(*args)
+    o, lse = ops.packed_attn_fwd(q, q, q, s, 2, 2, 64)
+    with pytest.raises(ValueError):
+        ops.packed_attn_bwd(o, q, q, q, o, lse, s, 2, 2, 64, dq=torch.empty_like(q))
+    with pytest.raises(ValueError):
+        ops.packed_attn_bwd(o, q, q, q, o, lse, s, 2, 2, 64, dq=q, dk=torch.empty_like(q), dv=torch.empty_like(q))
+
+
+def test_autograd_takes_any_strides():
+    T, H, D = 70, 2, 64
+    s = ops.pack_sequences(_cu([30, 40]), T, device=DEV)
+    x = [torch.randn(H * D, T, device=DEV).to(torch.bfloat16).t().requires_grad_(True) for _ in range(3)]
+    o = ops.packed_attention(*x, s, H, H, D)
+    g = torch.autograd.grad(o, x, torch.ones(1, 1, device=DEV, dtype=torch.bfloat16).expand(T, H * D))
+    want = attention(*[t.detach() for t in x], [30, 40], H, H, D, D ** -0.5,
+                     torch.ones(T, H * D, device=DEV))
+    for name, t in zip(("o", "dq", "dk", "dv"), (o.detach(), *g)):
+        within(t, want[name], name)
+
+
+def test_two_runs_are_equal_and_streams():
+    lens, Hq, Hkv, D = [400, 123, 300], 8, 2, 128
+    T = sum(lens)
+    q, k, v, do = _inputs(T, Hq, Hkv, D, seed=9)
+    s = ops.pack_sequences(_cu(lens), T, device=DEV)
+
+    def go():
+        o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D)
+        return (o, *ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D))
+    a = go()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b = go()
+    torch.cuda.current_stream().wait_stream(side)
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+
+
+def test_captured_step_replays_on_new_batches():
+    """Table, forward and backward captured once; replays see new lengths and new values."""
+    Hq, Hkv, D, T = 4, 2, 64, 300
+    batches = [([100, 150, 0], 1), ([10, 5, 280], 2), ([299, 0, 1], 3), ([0, 0, 0], 4)]
+    cu = torch.zeros(4, dtype=torch.int64, device=DEV)
+    buf = torch.zeros(T, (Hq + 2 * Hkv) * D, dtype=torch.bfloat16, device=DEV)
+    do = torch.zeros(T, Hq * D, dtype=torch.bfloat16, device=DEV)
+    q, k, v = buf[:, :Hq * D], buf[:, Hq * D:(Hq + Hkv) * D], buf[:, (Hq + Hkv) * D:]
+
+    def go():
+        s = ops.pack_sequences(cu, T)
+        o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D)
+        return (o, *ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D))
+
+    def load(lens, seed):
+        cu.copy_(_cu(lens))
+        gen = torch.Generator().manual_seed(seed)
+        buf.copy_(torch.randn(buf.shape, generator=gen))
+        do.copy_(torch.randn(do.shape, generator=gen))
+    load(*batches[0])
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        go()
+    torch.cuda.current_stream().wait_stream(st)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = go()
+    for b in batches[1:] + batches[:1]:
+        load(*b)
+        g.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in outs]
+        for x, y in zip(got, go()):
+            assert torch.equal(x, y)
