@@ -5,6 +5,7 @@ CPU tensors take the fp32 PyTorch reference path.
 """
 from . import _lib  # noqa: F401
 from .attention import attn_bwd, attn_fwd, flash_attention  # noqa: F401
+from .embedding import embedding, embedding_bwd, embedding_fwd  # noqa: F401
 from .fused import (bias_gelu, bias_gelu_bwd, bias_gelu_fwd, ce_stats,  # noqa: F401
                     cross_entropy, cross_entropy_fwd_bwd, embed_bwd, embed_fwd, pos_embed_bwd)
 from .norm import (bda_norm_fwd, colsum, layer_norm, layernorm_fwd, norm_bwd,  # noqa: F401

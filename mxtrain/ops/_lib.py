@@ -116,6 +116,10 @@ SIGNATURES = {
     "mx_packed_plan": [P, I, I, I, P, P, P, P, P],
     "mx_packed_attn_fwd": [P, P, P, I, I, I, P, I, P, P, P, P, I, I, I, I, F, I, P],
     "mx_packed_attn_bwd": [P, P, P, I, I, I, P, I, P, I, P, P, P, I, P, P, I, I, P, P, P, I, I, I, I, F, I, P],
+    # embedding.hip
+    "mx_embedding_fwd": [P, P, I64, I, F, P, P, I, P, I, I, P],
+    "mx_embedding_bwd_words": [I, I, I],
+    "mx_embedding_bwd": [P, I64, P, I, P, I, I, I, F, I, P, I64, P],
     # rope.hip
     "mx_rope": [P, I64, I, I, I, I, I, I, I, P, P, P, I, P],
     # vision.hip
