@@ -35,6 +35,7 @@ struct GArgs {
   int M, N, K;
   int tiles_m, tiles_n, gm;
   int act, accumulate;
+  int splits, nks;       // EPI 4: K-steps per split
 };
 
 __device__ __forceinline__ float act_fwd(int act, float x) {
@@ -97,6 +98,7 @@ __device__ __forceinline__ i32x4_t tile_rsrc(const uint16_t* base, int rows, int
 }
 
 // EPI 0: C (+)= acc   1: C = acc + bias   2: gate (two column halves)   3: gate gradient
+//     4: fp32 partial of one K range into part[split][M][N] (joined by gated_join_kernel)
 template <bool AKC, bool BKC, int WM, int WN, int FM, int FN, int BKT, int NSLOT, int MINB, int EPI>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(MINB, MINB))) void gated_gemm_kernel(
     const GArgs g) {
@@ -111,12 +113,17 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(MI
   const int G = lane >> 4, i = lane & 15;
   const int wm = wave / WN, wn = wave % WN;
   // XCD-contiguous order over groups of gm row tiles
-  const int wg = xcd_remap(blockIdx.x, gridDim.x);
+  // (the splits of a tile are adjacent ids)
+  const int wgs = xcd_remap(blockIdx.x, gridDim.x);
+  const int split = EPI == 4 ? wgs % g.splits : 0, wg = EPI == 4 ? wgs / g.splits : wgs;
   const int per = g.gm * g.tiles_n, grp = wg / per, rem = wg - grp * per;
   const int gmr = min(g.gm, g.tiles_m - grp * g.gm);   // (the last group may be smaller)
   const int tm = grp * g.gm + rem % gmr, tn = rem / gmr;
   const int m0 = tm * BM, n0 = tn * BNO;
-  const int K = g.K, nk = (K + BKT - 1) / BKT;
+  const int nk_all = (g.K + BKT - 1) / BKT;
+  const int kt0 = EPI == 4 ? split * g.nks : 0;     // first K-step
+  const int nk = EPI == 4 ? min(g.nks, nk_all - kt0) : nk_all;
+  const int K = g.K;
 
   // per-lane byte offsets of the DMA pieces inside one step's image source
   uint32_t voA[PA], voB[PB];
@@ -155,7 +162,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(MI
   const uint32_t lds0 = lds_addr(smem);
   const uint32_t ldsA = uni(lds0 + PA * wave * 1024), ldsB = uni(lds0 + IA + PB * wave * 1024);
   auto piece = [&](int slot, int it, int j) __attribute__((always_inline)) {
-    const int k0 = it * BKT;
+    const int k0 = (kt0 + it) * BKT;
     if (j < PA) {
       i32x4_t r;
       uint32_t vo = voA[j];
@@ -257,6 +264,21 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(MI
 
   // ---- epilogue: lane holds C[m][n + e], m = m0 + 16 (FM wm + s) + i, n = .. + 16 u + 4 G; pairs of
   // subtiles are re-dealt so that a lane stores 8 consecutive columns (16 B)
+  if constexpr (EPI == 4) {
+    float* P = g.part + (size_t)split * g.M * g.N;
+#pragma unroll
+    for (int s = 0; s < FM; ++s) {
+      const int m = m0 + 16 * (FM * wm + s) + i;
+#pragma unroll
+      for (int u = 0; u < FN; ++u) {
+        const int col = n0 + 16 * (FN * wn + u) + 4 * G;
+        if (m < g.M && col < g.N)
+          *reinterpret_cast<float4*>(P + (size_t)m * g.N + col) =
+              make_float4(acc[s][u][0], acc[s][u][1], acc[s][u][2], acc[s][u][3]);
+      }
+    }
+    return;
+  }
   constexpr int FO = DUAL ? FN / 2 : FN;
   const int colw = n0 + 16 * FO * wn, N = g.N;
   const int mrow = m0 + 16 * FM * wm + i;
@@ -278,37 +300,53 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(MI
     deal(v[0][0], v[0][1], v[1][0], v[1][1]);
     if (ok) *reinterpret_cast<uint4*>(p) = make_uint4(v[0][0], v[0][1], v[1][0], v[1][1]);
   };
-  auto get = [&](const uint16_t* p, uint32_t (&v)[2][2], bool ok) __attribute__((always_inline)) {
-    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-    if (ok) x = *reinterpret_cast<const uint4*>(p);
+  auto get = [&](const uint4& x, uint32_t (&v)[2][2]) __attribute__((always_inline)) {
     v[0][0] = x.x; v[0][1] = x.y; v[1][0] = x.z; v[1][1] = x.w;
     undeal(v[0][0], v[0][1], v[1][0], v[1][1]);
   };
+  // what the epilogue reads (pre; C when it accumulates) is fetched a row group ahead: one group's
+  // loads waited for in turn were 30 us of a 60 us launch (4096 x 1024 x 2688, 256 x 256 tiles)
+  constexpr int NR = EPI == 3 ? 2 : EPI == 0 ? 1 : 0;
+  uint4 pf[NR ? NR : 1][FO / 2];
+  auto fetch_row = [&](int s) __attribute__((always_inline)) {
+    const int m = mrow + 16 * s;
+#pragma unroll
+    for (int up = 0; up < FO / 2; ++up) {
+      const int col = colw + 32 * up + 8 * G;
+#pragma unroll
+      for (int h = 0; h < NR; ++h) {
+        pf[h][up] = make_uint4(0u, 0u, 0u, 0u);
+        if (m < g.M && col < N && (EPI == 3 || g.accumulate))
+          pf[h][up] = *reinterpret_cast<const uint4*>(EPI == 3 ? g.aux + (size_t)m * 2 * N + h * N + col
+                                                               : g.c + (size_t)m * g.ldc + col);
+      }
+    }
+  };
+  fetch_row(0);
 #pragma unroll
   for (int s = 0; s < FM; ++s) {
     const int m = mrow + 16 * s;
+    uint4 cur[NR ? NR : 1][FO / 2];
+#pragma unroll
+    for (int up = 0; up < FO / 2; ++up)
+#pragma unroll
+      for (int h = 0; h < NR; ++h) cur[h][up] = pf[h][up];
+    if (s + 1 < FM) fetch_row(s + 1);
 #pragma unroll
     for (int up = 0; up < FO / 2; ++up) {
       const int col = colw + 32 * up + 8 * G;       // the lane's 8 columns after the re-deal
       const bool ok = m < g.M && col < N;
       uint32_t c[2][2], pa[2][2], pb[2][2];
-      if constexpr (EPI == 0) {
-        if (g.accumulate) get(g.c + (size_t)m * g.ldc + col, pa, ok);
-      }
-      if constexpr (EPI == 3) {
-        get(g.aux + (size_t)m * 2 * N + col, pa, ok);
-        get(g.aux + (size_t)m * 2 * N + N + col, pb, ok);
-      }
+      if constexpr (NR > 0) get(cur[0][up], pa);
+      if constexpr (NR > 1) get(cur[NR - 1][up], pb);
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const int u = 2 * up + hf;
         float v[4], w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = acc[s][u][e] + bias[u][e];
-        if constexpr (EPI == 0) {
-          if (g.accumulate) {
-            v[0] += lo_bf(pa[hf][0]); v[1] += hi_bf(pa[hf][0]); v[2] += lo_bf(pa[hf][1]); v[3] += hi_bf(pa[hf][1]);
-          }
+        if constexpr (EPI == 0) {   // (zeros unless it accumulates)
+          v[0] += lo_bf(pa[hf][0]); v[1] += hi_bf(pa[hf][0]); v[2] += lo_bf(pa[hf][1]); v[3] += hi_bf(pa[hf][1]);
         }
         if constexpr (EPI == 2) {
 #pragma unroll
@@ -367,23 +405,202 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(MI
   }
 }
 
-template <bool AKC, bool BKC, int WM, int WN, int FM, int FN, int BKT, int NSLOT, int MINB, int EPI>
+// ---- few tokens (a decoding step): y^T = W x^T with the weight rows streamed once from memory.
+// A workgroup takes 16 output columns (of both halves for the gate) and its NW waves split K, so
+// that even a 1024-column product has hundreds of waves with all their loads in flight; no LDS on
+// the way in (a weight is used once), partial sums meet in LDS.  Lane (G, i) loads row i, k 8G ..
+// 8G + 7 of a 16 x 32 block; NG groups of 16 tokens.
+template <int NG, bool DUAL, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void gated_few_kernel(const GArgs g) {
+  constexpr int NH = DUAL ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) float4 red[NW][NH * NG][64];
+  const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), G = lane >> 4, i = lane & 15;
+  const int n0 = blockIdx.x * 16, N = g.N, K = g.K, M = g.M;
+  const int steps = (K + 31) / 32, per = (steps + NW - 1) / NW;
+  const int s0 = w * per, s1 = min(steps, s0 + per);
+  const uint16_t* wp[NH];
+#pragma unroll
+  for (int h = 0; h < NH; ++h) wp[h] = g.b + (size_t)(min(n0 + i, N - 1) + h * N) * g.ldb;
+  const uint16_t* xp[NG];
+#pragma unroll
+  for (int t = 0; t < NG; ++t) xp[t] = g.a + (size_t)min(16 * t + i, M - 1) * g.lda;
+  f32x4 acc[NH][NG];
+#pragma unroll
+  for (int h = 0; h < NH; ++h)
+#pragma unroll
+    for (int t = 0; t < NG; ++t) acc[h][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto load = [&](const uint16_t* p, int k) __attribute__((always_inline)) {   // zeros past K
+    const uint4 v = *reinterpret_cast<const uint4*>(p + (k < K ? k : 0));
+    const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+    return __builtin_bit_cast(bf16x8, k < K ? v : z);
+  };
+  auto block = [&](int s, auto unc) __attribute__((always_inline)) {   // UN steps, every load in flight
+    constexpr int UN = decltype(unc)::value;
+    bf16x8 a[UN][NH], b[UN][NG];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int k = 32 * (s + u) + 8 * G;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) a[u][h] = load(wp[h], k);
+#pragma unroll
+      for (int t = 0; t < NG; ++t) b[u][t] = load(xp[t], k);
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int t = 0; t < NG; ++t) acc[h][t] = mfma16(a[u][h], b[u][t], acc[h][t]);
+  };
+  int s = s0;
+  for (; s + 4 <= s1; s += 4) block(s, std::integral_constant<int, 4>{});
+  if (s + 2 <= s1) {
+    block(s, std::integral_constant<int, 2>{});
+    s += 2;
+  }
+  if (s < s1) block(s, std::integral_constant<int, 1>{});
+#pragma unroll
+  for (int h = 0; h < NH; ++h)
+#pragma unroll
+    for (int t = 0; t < NG; ++t)
+      red[w][h * NG + t][lane] = make_float4(acc[h][t][0], acc[h][t][1], acc[h][t][2], acc[h][t][3]);
+  __syncthreads();
+  // wave t finishes token group t: lane holds columns n0 + 4 G .. + 3 of token 16 t + i
+  if (w >= NG) return;
+  const int m = 16 * w + i, col = n0 + 4 * G;
+  float v[NH][4];
+#pragma unroll
+  for (int h = 0; h < NH; ++h) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[h][e] = 0.f;
+#pragma unroll
+    for (int q = 0; q < NW; ++q) {
+      const float4 x = red[q][h * NG + w][lane];
+      v[h][0] += x.x; v[h][1] += x.y; v[h][2] += x.z; v[h][3] += x.w;
+    }
+  }
+  if (m >= M || col >= N) return;
+  if (g.bias) {
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      const uint2 x = *reinterpret_cast<const uint2*>(g.bias + h * N + col);
+      v[h][0] += lo_bf(x.x); v[h][1] += hi_bf(x.x); v[h][2] += lo_bf(x.y); v[h][3] += hi_bf(x.y);
+    }
+  }
+  if constexpr (DUAL) {
+    if (g.aux) {
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+        *reinterpret_cast<uint2*>(g.aux + (size_t)m * 2 * N + h * N + col) =
+            make_uint2(pack2(v[h][0], v[h][1]), pack2(v[h][2], v[h][3]));
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[0][e] = act_fwd(g.act, v[0][e]) * v[NH - 1][e];
+  }
+  *reinterpret_cast<uint2*>(g.c + (size_t)m * g.ldc + col) =
+      make_uint2(pack2(v[0][0], v[0][1]), pack2(v[0][2], v[0][3]));
+}
+constexpr int kFewTokens = 64;
+template <bool DUAL>
+int run_few(const GArgs& g, hipStream_t s) {
+  const dim3 grid((g.N + 15) / 16);
+  constexpr int NW = DUAL ? 8 : 16;
+  if (g.M <= 16) hipLaunchKernelGGL((gated_few_kernel<1, DUAL, NW>), grid, dim3(64 * NW), 0, s, g);
+  else if (g.M <= 32) hipLaunchKernelGGL((gated_few_kernel<2, DUAL, NW>), grid, dim3(64 * NW), 0, s, g);
+  else hipLaunchKernelGGL((gated_few_kernel<4, DUAL, NW>), grid, dim3(64 * NW), 0, s, g);
+  return hipGetLastError();
+}
+
+// sums the partials of EPI 4 in order: C = sum (+ bias) (+ C)
+__global__ __launch_bounds__(256) void gated_join_kernel(const GArgs g) {
+  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int nv = g.N / 8;
+  if (v >= (int64_t)g.M * nv) return;
+  const int64_t m = v / nv;
+  const int n = (int)(v - m * nv) * 8;
+  float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int k = 0; k < g.splits; ++k) {
+    const float4* p = reinterpret_cast<const float4*>(g.part + ((size_t)k * g.M + m) * g.N + n);
+    const float4 x = p[0], y = p[1];
+    o[0] += x.x; o[1] += x.y; o[2] += x.z; o[3] += x.w;
+    o[4] += y.x; o[5] += y.y; o[6] += y.z; o[7] += y.w;
+  }
+  uint16_t* c = g.c + (size_t)m * g.ldc + n;
+  float x[8];
+  if (g.bias) {
+    unpack8(*reinterpret_cast<const uint4*>(g.bias + n), x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] += x[j];
+  }
+  if (g.accumulate) {
+    unpack8(*reinterpret_cast<const uint4*>(c), x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] += x[j];
+  }
+  *reinterpret_cast<uint4*>(c) = pack8(o);
+}
+
+template <bool AKC, bool BKC, int WM, int WN, int FM, int FN, int BKT, int NSLOT, int EPI>
 int launch(GArgs g, hipStream_t s) {
   using Gm = Geo<AKC, BKC, WM, WN, FM, FN, BKT, NSLOT>;
   const int bn = EPI == 2 ? Gm::BN / 2 : Gm::BN;
   g.tiles_m = (g.M + Gm::BM - 1) / Gm::BM;
   g.tiles_n = (g.N + bn - 1) / bn;
   g.gm = 8;
-  if ((int64_t)g.tiles_m * g.tiles_n >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((gated_gemm_kernel<AKC, BKC, WM, WN, FM, FN, BKT, NSLOT, MINB, EPI>),
-                     dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(Gm::NT), 0, s, g);
+  const int nk = (g.K + BKT - 1) / BKT;
+  g.nks = (nk + g.splits - 1) / g.splits;
+  g.splits = (nk + g.nks - 1) / g.nks;              // (no empty split)
+  const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+  if (grid >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((gated_gemm_kernel<AKC, BKC, WM, WN, FM, FN, BKT, NSLOT, 2, EPI>), dim3((unsigned)grid),
+                     dim3(Gm::NT), 0, s, g);
+  if (EPI == 4) {
+    const int64_t vecs = (int64_t)g.M * (g.N / 8);
+    hipLaunchKernelGGL(gated_join_kernel, dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, s, g);
+  }
   return hipGetLastError();
 }
+
+// tiles: rows, columns of the product (the gate's two halves together), column-partial rows per tile
+struct Tile {
+  int bm, bn, wm;
+};
+constexpr Tile kTiles[] = {
+    {128, 128, 2},   // 0: 4 waves of 64 x 64, 64-deep steps, 2 slots: two workgroups per CU
+    {256, 256, 2},   // 1: 8 waves of 128 x 64, 64-deep steps, 2 slots
+    {256, 256, 2},   // 2: 8 waves of 128 x 64, 32-deep steps, 4 slots
+    {128, 128, 4},   // 3: 8 waves of 32 x 64, 64-deep steps, 4 slots
+    {256, 128, 4},   // 4: 8 waves of 64 x 64, 64-deep steps, 3 slots
+};
+constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
+
 template <bool AKC, bool BKC, int EPI>
-int run(const GArgs& g, hipStream_t s) {
-  return launch<AKC, BKC, 2, 2, 4, 4, 64, 2, 2, EPI>(g, s);
+int run_tile(int tile, const GArgs& g, hipStream_t s) {
+  switch (tile) {
+    case 0: return launch<AKC, BKC, 2, 2, 4, 4, 64, 2, EPI>(g, s);
+    case 1: return launch<AKC, BKC, 2, 4, 8, 4, 64, 2, EPI>(g, s);
+    case 2: return launch<AKC, BKC, 2, 4, 8, 4, 32, 4, EPI>(g, s);
+    case 3: return launch<AKC, BKC, 4, 2, 2, 4, 64, 4, EPI>(g, s);
+    case 4: return launch<AKC, BKC, 4, 2, 4, 4, 64, 3, EPI>(g, s);
+    default: return hipErrorInvalidValue;
+  }
 }
-constexpr int kPartRows = 64;   // rows behind one row of column partials (16 FM)
+// splits > 1: fp32 partials in `part` (splits x M x N) and a join
+template <bool AKC, bool BKC, int EPI>
+int run(int tile, int splits, GArgs g, hipStream_t s) {
+  if (splits < 1 || splits > 64) return hipErrorInvalidValue;
+  g.splits = splits;
+  if constexpr (EPI == 0 || EPI == 1) {
+    if (splits > 1) {
+      if (!g.part || ((uintptr_t)g.part & 15)) return hipErrorInvalidValue;
+      return run_tile<AKC, BKC, 4>(tile, g, s);
+    }
+  } else if (splits != 1) {
+    return hipErrorInvalidValue;
+  }
+  return run_tile<AKC, BKC, EPI>(tile, g, s);
+}
 
 bool bad_rows(const void* p, int ld, int cols) {   // 16-B rows; tile offsets stay below 2^31 bytes
   return p == nullptr || ((uintptr_t)p & 15) || (ld & 7) || ld < cols || ld > (1 << 21);
@@ -392,9 +609,15 @@ bool bad_dim(int n) { return n <= 0 || (n & 7) || n > (1 << 20); }
 
 }  // namespace
 
+// geometry of a tile: what = 0 rows, 1 columns, 2 column-partial rows (mx_gated_dgate); -1: no such tile
+MX_EXPORT int mx_gated_tile(int tile, int what) {
+  if (tile < 0 || tile >= kNumTiles) return -1;
+  return what == 0 ? kTiles[tile].bm : what == 1 ? kTiles[tile].bn : kTiles[tile].wm;
+}
+
 // h[M][F] = act(x W1a^T + b1a) (x W1b^T + b1b): x [M][ldx] (K wide), w1 [2F][ldw]; pre [M][2F] or null
 MX_EXPORT int mx_gated_fwd(const void* x, int ldx, const void* w1, int ldw, const void* b1, void* pre, void* h, int M,
-                           int K, int F, int act, hipStream_t s) {
+                           int K, int F, int act, int tile, hipStream_t s) {
   if (M <= 0 || bad_dim(K) || bad_dim(F) || bad_rows(x, ldx, K) || bad_rows(w1, ldw, K) || bad_rows(h, F, F) ||
       ((uintptr_t)pre & 15) || ((uintptr_t)b1 & 15) || act < 0 || act > 1)
     return hipErrorInvalidValue;
@@ -403,59 +626,59 @@ MX_EXPORT int mx_gated_fwd(const void* x, int ldx, const void* w1, int ldw, cons
   g.bias = (const uint16_t*)b1;
   g.lda = ldx; g.ldb = ldw; g.ldc = F;
   g.M = M; g.N = F; g.K = K; g.act = act;
-  return run<true, true, 2>(g, s);
+  if (M <= kFewTokens) return run_few<true>(g, s);
+  return run<true, true, 2>(tile, 1, g, s);
 }
 
-// y[M][N] = h W2^T (+ b2): h [M][K] contiguous, w2 [N][ldw]
+// y[M][N] = h W2^T (+ b2): h [M][K] contiguous, w2 [N][ldw]; part: splits x M x N floats (splits > 1)
 MX_EXPORT int mx_gated_down(const void* h, const void* w2, int ldw, const void* b2, void* y, int M, int N, int K,
-                            hipStream_t s) {
+                            int tile, int splits, float* part, hipStream_t s) {
   if (M <= 0 || bad_dim(K) || bad_dim(N) || bad_rows(h, K, K) || bad_rows(w2, ldw, K) || bad_rows(y, N, N) ||
       ((uintptr_t)b2 & 15))
     return hipErrorInvalidValue;
   GArgs g{};
   g.a = (const uint16_t*)h; g.b = (const uint16_t*)w2; g.c = (uint16_t*)y; g.bias = (const uint16_t*)b2;
-  g.lda = K; g.ldb = ldw; g.ldc = N;
+  g.lda = K; g.ldb = ldw; g.ldc = N; g.part = part;
   g.M = M; g.N = N; g.K = K;
-  return run<true, true, 1>(g, s);
+  if (M <= kFewTokens) return run_few<false>(g, s);
+  return run<true, true, 1>(tile, splits, g, s);
 }
 
-// rows of column partials mx_gated_dgate writes for M tokens
-MX_EXPORT int mx_gated_parts(int M) { return (M + 127) / 128 * 2; }
-
-// dpre[M][2F] = [dh b act'(a) | dh act(a)], dh = dy W2: dy [M][lddy] (K wide), w2 [K][ldw]; part or null
+// dpre[M][2F] = [dh b act'(a) | dh act(a)], dh = dy W2: dy [M][lddy] (K wide), w2 [K][ldw]; part null or
+// the fp32 column partials [tiles x mx_gated_tile(tile, 2)][2F]
 MX_EXPORT int mx_gated_dgate(const void* dy, int lddy, const void* w2, int ldw, const void* pre, void* dpre,
-                             float* part, int M, int K, int F, int act, hipStream_t s) {
+                             float* part, int M, int K, int F, int act, int tile, hipStream_t s) {
   if (M <= 0 || bad_dim(K) || bad_dim(F) || bad_rows(dy, lddy, K) || bad_rows(w2, ldw, F) ||
       bad_rows(pre, 2 * F, 2 * F) || bad_rows(dpre, 2 * F, 2 * F) || ((uintptr_t)part & 15) || act < 0 || act > 1)
     return hipErrorInvalidValue;
-  static_assert(kPartRows * 2 == 128, "mx_gated_parts counts two partial rows per 128-row tile");
   GArgs g{};
   g.a = (const uint16_t*)dy; g.b = (const uint16_t*)w2; g.aux = (uint16_t*)const_cast<void*>(pre);
   g.grad = (uint16_t*)dpre; g.part = part;
   g.lda = lddy; g.ldb = ldw;
   g.M = M; g.N = F; g.K = K; g.act = act;
-  return run<true, false, 3>(g, s);
+  return run<true, false, 3>(tile, 1, g, s);
 }
 
 // dx[M][N] = dpre W1: dpre [M][K] contiguous, w1 [K][ldw]
-MX_EXPORT int mx_gated_dx(const void* dpre, const void* w1, int ldw, void* dx, int M, int N, int K, hipStream_t s) {
+MX_EXPORT int mx_gated_dx(const void* dpre, const void* w1, int ldw, void* dx, int M, int N, int K, int tile,
+                          int splits, float* part, hipStream_t s) {
   if (M <= 0 || bad_dim(K) || bad_dim(N) || bad_rows(dpre, K, K) || bad_rows(w1, ldw, N) || bad_rows(dx, N, N))
     return hipErrorInvalidValue;
   GArgs g{};
   g.a = (const uint16_t*)dpre; g.b = (const uint16_t*)w1; g.c = (uint16_t*)dx;
-  g.lda = K; g.ldb = ldw; g.ldc = N;
+  g.lda = K; g.ldb = ldw; g.ldc = N; g.part = part;
   g.M = M; g.N = N; g.K = K;
-  return run<true, false, 0>(g, s);
+  return run<true, false, 0>(tile, splits, g, s);
 }
 
 // dw[M][N] (+)= a^T b over T rows: a [T][lda] (M wide), b [T][ldb] (N wide), dw [M][ldc]
 MX_EXPORT int mx_gated_dw(const void* a, int lda, const void* b, int ldb, void* dw, int ldc, int T, int M, int N,
-                          int accumulate, hipStream_t s) {
+                          int accumulate, int tile, int splits, float* part, hipStream_t s) {
   if (T <= 0 || bad_dim(M) || bad_dim(N) || bad_rows(a, lda, M) || bad_rows(b, ldb, N) || bad_rows(dw, ldc, N))
     return hipErrorInvalidValue;
   GArgs g{};
   g.a = (const uint16_t*)a; g.b = (const uint16_t*)b; g.c = (uint16_t*)dw;
-  g.lda = lda; g.ldb = ldb; g.ldc = ldc;
+  g.lda = lda; g.ldb = ldb; g.ldc = ldc; g.part = part;
   g.M = M; g.N = N; g.K = T; g.accumulate = accumulate;
-  return run<false, false, 0>(g, s);
+  return run<false, false, 0>(tile, splits, g, s);
 }

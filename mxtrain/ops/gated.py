@@ -84,6 +84,50 @@ def _check(name, act, x, w1, b1, w2, b2, **more):
     return T, H, F, Ho, hip
 
 
+# ------------------------------------------------------------------ tiles
+# Per tile of csrc/gated.hip: (rows, columns, workgroups per CU, us per 64-deep step, us per round of
+# workgroups beside the steps), fitted to one MI355X over 4096 x 4096 x 10880 (steps) and
+# 4096 x 1024 x 2688 (rounds); a round is one workgroup on every slot of the 256 CUs.
+_TILES = ((128, 128, 2, 1.14, 5.0), (256, 256, 1, 1.69, 8.0), (256, 256, 1, 1.72, 5.0), (128, 128, 1, 0.62, 4.0),
+          (256, 128, 1, 0.985, 5.0))
+_PLANS = {}
+
+
+def _plan(kind, M, N, K):
+    """(tile, splits) of one product, M x N over K (N: columns of both halves for "gate"): the
+    least estimated time.  Big tiles move the fewest operand bytes per product, so they win where
+    they fill whole rounds (4096 x 4096 x 10880 "down": 287 us with 256 x 256 tiles, 387 with 128 x
+    128); few tiles leave CUs idle, so smaller ones with a deeper ring win (1003 x 768 x 2048 "gate":
+    12.6 us against 24.9), and a long K is split once the tiles cover less than half of the chip
+    (its "dx": 21.2 us in 4 splits, 40 us in one)."""
+    key = (kind, M, N, K)
+    best = _PLANS.get(key)
+    if best is None:
+        steps, cost = -(-K // 64), None
+        for tile, (bm, bn, per, step, fix) in enumerate(_TILES):
+            tiles = -(-M // bm) * -(-N // bn)
+            for splits in ((1, 2, 4, 8) if kind in ("down", "dx", "dw") else (1,)):
+                if splits > 1 and (tiles * splits > 256 or steps < 8 * splits):
+                    break
+                wgs = tiles * splits
+                rounds = -(-wgs // (256 * per))
+                if per == 2 and wgs <= 256:      # alone on its CU: the two-slot ring waits for memory
+                    step = 0.97
+                est = rounds * (-(-steps // splits) * step + fix)
+                if splits > 1:                   # partials written and read, one more launch
+                    est += 4.0 + splits * M * N * 8 / 4e6
+                if cost is None or est < cost:
+                    cost, best = est, (tile, splits)
+        if len(_PLANS) > 4096:
+            _PLANS.clear()
+        _PLANS[key] = best
+    return best
+
+
+def _split_ws(splits, M, N, device):
+    return torch.empty(splits * M * N, dtype=torch.float32, device=device) if splits > 1 else None
+
+
 # ------------------------------------------------------------------ forward / backward
 def gated_mlp_fwd(x, w1, b1, w2, b2, act: str = "silu", save: bool = True):
     """x [T, H] -> (y [T, Ho], pre [T, 2F], h [T, F]); without ``save`` the last two are None.
@@ -105,9 +149,11 @@ def gated_mlp_fwd(x, w1, b1, w2, b2, act: str = "silu", save: bool = True):
         pre = torch.empty(T, 2 * F, dtype=x.dtype, device=x.device) if save else None
         if T:
             _lib.call("mx_gated_fwd", _lib.ptr(x), _ld(x), _lib.ptr(w1), _ld(w1), _lib.ptr(b1), _lib.ptr(pre),
-                      _lib.ptr(h), T, H, F, ACTS[act], _lib.stream())
+                      _lib.ptr(h), T, H, F, ACTS[act], _plan("gate", T, 2 * F, H)[0], _lib.stream())
+            tile, splits = _plan("down", T, Ho, F)
+            part = _split_ws(splits, T, Ho, x.device)
             _lib.call("mx_gated_down", _lib.ptr(h), _lib.ptr(w2), _ld(w2), _lib.ptr(b2), _lib.ptr(y), T, Ho, F,
-                      _lib.stream())
+                      tile, splits, _lib.ptr(part), _lib.stream())
     return (y, pre, h) if save else (y, None, None)
 
 
@@ -161,20 +207,27 @@ def gated_mlp_bwd(dy, x, pre, h, w1, b1, w2, b2, act: str = "silu", dw1=None, db
         s = _lib.stream()
         dpre = torch.empty(T, 2 * F, dtype=x.dtype, device=x.device)
         part = buf = None
-        nparts = _lib.query("mx_gated_parts", T)
+        tile, _ = _plan("dgate", T, F, Ho)
+        bm = _lib.query("mx_gated_tile", tile, 0)
+        nparts = (T + bm - 1) // bm * _lib.query("mx_gated_tile", tile, 2)
         if db1 is not None:
             part, buf = colsum_partials_buffer(nparts, 2 * F, x.device)
         _lib.call("mx_gated_dgate", _lib.ptr(dy), _ld(dy), _lib.ptr(w2), _ld(w2), _lib.ptr(pre), _lib.ptr(dpre),
-                  _lib.ptr(part), T, Ho, F, ACTS[act], s)
+                  _lib.ptr(part), T, Ho, F, ACTS[act], tile, s)
         dx = None
         if need_dx:
             dx = torch.empty(T, H, dtype=x.dtype, device=x.device)
-            _lib.call("mx_gated_dx", _lib.ptr(dpre), _lib.ptr(w1), _ld(w1), _lib.ptr(dx), T, H, 2 * F, s)
+            tile, splits = _plan("dx", T, H, 2 * F)
+            ws = _split_ws(splits, T, H, x.device)
+            _lib.call("mx_gated_dx", _lib.ptr(dpre), _lib.ptr(w1), _ld(w1), _lib.ptr(dx), T, H, 2 * F, tile, splits,
+                      _lib.ptr(ws), s)
         if need_dw:
-            _lib.call("mx_gated_dw", _lib.ptr(dpre), 2 * F, _lib.ptr(x), _ld(x), _lib.ptr(dw1), _ld(dw1), T, 2 * F, H,
-                      int(accumulate), s)
-            _lib.call("mx_gated_dw", _lib.ptr(dy), _ld(dy), _lib.ptr(h), F, _lib.ptr(dw2), _ld(dw2), T, Ho, F,
-                      int(accumulate), s)
+            for a, b, out in ((dpre, x, dw1), (dy, h, dw2)):
+                (m, n) = out.shape
+                tile, splits = _plan("dw", m, n, T)
+                ws = _split_ws(splits, m, n, x.device)
+                _lib.call("mx_gated_dw", _lib.ptr(a), _ld(a), _lib.ptr(b), _ld(b), _lib.ptr(out), _ld(out), T, m, n,
+                          int(accumulate), tile, splits, _lib.ptr(ws), s)
             if db1 is not None:
                 colsum_finalize(buf, nparts, 2 * F, db1, accumulate)
             if db2 is not None:
