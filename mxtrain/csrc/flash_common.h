@@ -104,8 +104,7 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& acc, int base) {
 // caller maps rank 0 to the heaviest causal block), and, when the head count is a multiple
 // of 8, every block of a head on one XCD (workgroups are dealt round-robin over the 8 XCDs,
 // id % 8): its K/V (Q/dO) stream is then read once into that XCD's L2.
-__device__ __forceinline__ void block_map(int nheads, int& rank, int& head) {
-  const int L = blockIdx.x;
+__device__ __forceinline__ void block_map(int L, int nheads, int& rank, int& head) {
   if ((nheads & 7) == 0) {
     const int x = L & 7, idx = L >> 3, nh8 = nheads >> 3;
     rank = idx / nh8;
@@ -114,6 +113,10 @@ __device__ __forceinline__ void block_map(int nheads, int& rank, int& head) {
     rank = L / nheads;
     head = L - rank * nheads;
   }
+}
+
+__device__ __forceinline__ void block_map(int nheads, int& rank, int& head) {
+  block_map((int)blockIdx.x, nheads, rank, head);
 }
 
 }  // namespace flash

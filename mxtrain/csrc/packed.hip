@@ -67,6 +67,8 @@ struct PArgs {
   int ldq, ldk, ldv, lddo, ldo, ldout, lddk, lddv;
   int T, Hq, Hkv;
   float c, scale;               // scale log2(e), scale
+  float* part;                  // D = 128: partial dK / dV of split blocks
+  int nsplit;
   int fill;                     // zero the rows behind the last sequence (else leave them)
 };
 
@@ -409,10 +411,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 }
 
 // ============================================================================ key-major
-// dK, dV.  Four waves of 32 keys, key on the MFMA lane; Q / dO tiles of QT rows (and their lse,
+// dK, dV, D = 64.  Four waves of 32 keys, key on the MFMA lane; Q / dO tiles of QT rows (and their lse,
 // delta) stream through a two-slot LDS-DMA ring, over the query heads of the key head's group.
 template <int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1))) void
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void
 packed_kmajor_kernel(const PArgs a) {
   constexpr int KB = 128, QT = 64, NQS = QT / 32, NKK = D / 16, NDT = D / 32;
   constexpr int RB = D * 2, CPR = D / 8, RPP = 64 / CPR, TILE = QT * RB, PPW = TILE / 1024 / 4;
@@ -606,6 +608,336 @@ packed_kmajor_kernel(const PArgs a) {
   }
 }
 
+// D = 128.  Two 32-key groups per wave, one wave per SIMD: every Q / dO fragment read from LDS feeds
+// two MFMAs (a 32-key wave needs 1408 LDS cycles per 1024 MFMA cycles of the four SIMDs -- the
+// transposed reads run at half rate --, this one 1408 per 2048), and the accumulators of both groups
+// (256 registers), their K and V rows (128) and S, dP (64) just fit the 512 registers.
+// A workgroup holds 256 keys.  Blocks of long sequences are split along their (query head, query
+// tile) items over up to `nsplit` workgroups, whose fp32 partial sums packed_join_kernel adds in order.
+constexpr int KB2 = 256, QT2 = 64, SPLIT_MIN = 24;   // fewest items of a split
+__device__ __forceinline__ int block_splits(int items, int nsplit) { return max(1, min(nsplit, items / SPLIT_MIN)); }
+
+// MFMA with its accumulator in ordinary registers.  The compiler gives every MFMA of a kernel that
+// needs accumulation registers an accumulator there; dK and dV of 64 keys take all 256 of them, and
+// it moved S and dP in and out of them at every subtile.  Written as asm, so the wait between the
+// last product and the first use is mfma_v_done's: 8 passes of 4 cycles and 3 more are required,
+// 24 are waited.  A product's operands are read from LDS (waited for by the compiler) or long loaded.
+__device__ __forceinline__ void mfma_v_first(f32x16& d, bf16x8 a, bf16x8 b) {
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mfma_v(f32x16& d, bf16x8 a, bf16x8 b) {
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mfma_v_done(f32x16& a, f32x16& b, f32x16& c, f32x16& d) {
+  asm volatile("s_nop 15\n\ts_nop 7" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+}
+
+template <int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void packed_kmajor2_kernel(const PArgs a) {
+  constexpr int NL = 2;   // V fragments kept in LDS: those the registers do not hold
+  constexpr int QT = QT2, NQS = QT / 32, NKK = D / 16, NDT = D / 32;
+  constexpr int RB = D * 2, CPR = D / 8, RPP = 64 / CPR, TILE = QT * RB, PPW = TILE / 1024 / 4;
+  __shared__ __attribute__((aligned(16))) char ring[2][2 * TILE];   // Q, dO
+  __shared__ __attribute__((aligned(16))) float stat[2][2][64];     // lse, delta
+  __shared__ __attribute__((aligned(16))) uint4 vlds[4][2 * NL][64];  // the waves' V fragments of kk < NL
+  const int tid = threadIdx.x, lane = tid & 63, wl = uni(tid >> 6);
+  const int r = lane & 31, hh = lane >> 5, g = lane >> 4, gi = lane & 15;
+  const int T = a.T, nv = uni(a.meta[0]);
+  const int nblk = gridDim.x / a.nsplit, sp = blockIdx.x / nblk;
+  int rank, hk;
+  block_map(blockIdx.x - sp * nblk, a.Hkv, rank, hk);
+  const int grp = a.Hq / a.Hkv;
+  const int k0 = rank * KB2, kw = k0 + 64 * wl;
+  if (k0 >= nv) {
+    if (a.fill && sp == 0)
+      for (int key = kw + r; key < min(kw + 64, T); key += 32) {
+        zero_row<D>(a.dk + (size_t)key * a.lddk + hk * D, hh);
+        zero_row<D>(a.dv + (size_t)key * a.lddv + hk * D, hh);
+      }
+    return;
+  }
+  const int qend = uni(a.end[min(k0 + KB2, nv) - 1]);
+  const int nqt = (qend - k0 + QT - 1) / QT, items = nqt * grp;
+  const int nsp = block_splits(items, a.nsplit), per = (items + nsp - 1) / nsp;
+  const int t0 = sp * per, t1 = min(items, t0 + per);
+  if (sp >= nsp) return;
+  const bool wave_on = kw < nv;
+  const int klast = min(kw + 63, nv - 1);
+  const int emax = uni(a.end[max(klast, 0)]);
+  int key[2], cnt[2], emin[2];
+  bf16x8 kf[2][NKK], vf[2][NKK - NL];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    key[j] = kw + 32 * j + r;
+    const int kc = min(key[j], nv - 1);
+    cnt[j] = key[j] < nv ? a.end[kc] - key[j] : 0;     // rows that see this key: key .. key + cnt - 1
+    emin[j] = uni(a.end[min(kw + 32 * j, nv - 1)]);
+    const uint16_t* kp = a.k + (size_t)kc * a.ldk + hk * D + 8 * hh;
+    const uint16_t* vp = a.v + (size_t)kc * a.ldv + hk * D + 8 * hh;
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) {
+      kf[j][kk] = ld8(kp + 16 * kk);
+      if (kk < NL) vlds[wl][2 * kk + j][lane] = *reinterpret_cast<const uint4*>(vp + 16 * kk);
+      else vf[j][kk < NL ? 0 : kk - NL] = ld8(vp + 16 * kk);
+    }
+  }
+  f32x16 dvacc[2][NDT], dkacc[2][NDT];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) { dvacc[j][dt] = f32x16{}; dkacc[j][dt] = f32x16{}; }
+  __builtin_amdgcn_s_waitcnt(0);   // (see packed_qmajor_kernel)
+
+  // LDS offsets: chunk 2 kk + hh (row reads) and 4 dt + .. (transposed reads) differ from the first
+  // by bits that the swizzle only flips, so one register and a XOR stand for each table
+  static_assert(D == 128, "256-B rows");
+  // (made opaque where they are used, so that the XORs are not hoisted into registers there are not)
+  int offQ0 = toff<D>(r, hh);
+  const int tcol = 16 * (g & 1) + 4 * (gi & 3), trow = 4 * hh + (gi >> 2);
+  int offT0 = toff<D>(trow, tcol >> 3) + (tcol & 7) * 2, offT1 = toff<D>(trow + 8, tcol >> 3) + (tcol & 7) * 2;
+  auto rread = [&](const char* X, int kk) __attribute__((always_inline)) { return lds8(X, offQ0 ^ (kk << 5)); };
+  auto tread = [&](const char* X, int dt) __attribute__((always_inline)) {
+    return cat(tr_read(X, offT0 ^ (dt << 6)), tr_read(X, offT1 ^ (dt << 6)));
+  };
+  // DMA pieces of a wave are 16 rows apart (the same swizzle)
+  const int R0 = wl * RPP + lane / CPR, ch0 = (lane % CPR) ^ swz<D>(R0);
+  uint32_t voQ = (uint32_t)(R0 * a.ldq + ch0 * 8) * 2u, voO = (uint32_t)(R0 * a.lddo + ch0 * 8) * 2u;
+  auto issue = [&](char* qd, char* od, float* ld, float* dd, int hq, int qs) __attribute__((always_inline)) {
+    const int rows = min(QT, nv - qs);
+    asm volatile("" : "+v"(voQ), "+v"(voO));
+    const i32x4_t qr = rows_rsrc<D>(a.q + (size_t)qs * a.ldq + hq * D, rows, a.ldq);
+    const i32x4_t dr = rows_rsrc<D>(a.dout + (size_t)qs * a.lddo + hq * D, rows, a.lddo);
+#pragma unroll
+    for (int i = 0; i < PPW; ++i) {
+      dma16_buf(qr, voQ + (uint32_t)(8 * RPP * i * a.ldq), qd + (wl + 4 * i) * 1024);
+      dma16_buf(dr, voO + (uint32_t)(8 * RPP * i * a.lddo), od + (wl + 4 * i) * 1024);
+    }
+    if (wl < 2) {
+      const size_t li = (size_t)hq * T + min(qs + lane, nv - 1);
+      if (wl == 0) dma4(a.lse + li, (char*)ld);
+      else dma4(a.delta + li, (char*)dd);
+    }
+  };
+  const float c = a.c;
+  uint32_t bad = 0;   // (see packed_qmajor_kernel)
+  auto body = [&](const char* Qt, const char* Ot, const float* Lt, const float* Dt, int qs) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int u = 0; u < NQS; ++u) {
+      const int qsu = qs + 32 * u;
+      if (uni(qsu + 31 < kw || qsu >= emax ? 1 : 0)) continue;
+      asm volatile("" : "+v"(offQ0), "+v"(offT0), "+v"(offT1));
+      f32x16 s[2], dp[2];
+      const char* Qu = Qt + 32 * u * RB;
+      const char* Ou = Ot + 32 * u * RB;
+      // part: some (row, key) pair of the subtile is masked
+      const bool part = uni(qsu < kw + 63 || qsu + 32 > emin[0] || qsu + 32 > emin[1] || kw + 63 >= nv ? 1 : 0);
+      // one step's fragments are read under the step before; the barriers keep the compiler from reading
+      // all of them first (there are no registers left for that)
+      auto vread = [&](int x) __attribute__((always_inline)) { return __builtin_bit_cast(bf16x8, vlds[wl][x][lane]); };
+      bf16x8 fr[2][2] = {{rread(Qu, 0), rread(Ou, 0)}, {}};
+      bf16x8 vl[2][2] = {{vread(0), vread(1)}, {}};
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk) {
+        bf16x8 (&f)[2] = fr[kk & 1], (&n)[2] = fr[(kk & 1) ^ 1];
+        if (kk + 1 < NKK) {
+          n[0] = rread(Qu, kk + 1);
+          n[1] = rread(Ou, kk + 1);
+        }
+        if (kk + 1 < NL) {
+          vl[(kk & 1) ^ 1][0] = vread(2 * kk + 2);
+          vl[(kk & 1) ^ 1][1] = vread(2 * kk + 3);
+        }
+        const bf16x8 v0 = kk < NL ? vl[kk & 1][0] : vf[0][kk < NL ? 0 : kk - NL];
+        const bf16x8 v1 = kk < NL ? vl[kk & 1][1] : vf[1][kk < NL ? 0 : kk - NL];
+        if (kk == 0) {
+          mfma_v_first(s[0], f[0], kf[0][kk]);
+          mfma_v_first(dp[0], f[1], v0);
+          mfma_v_first(s[1], f[0], kf[1][kk]);
+          mfma_v_first(dp[1], f[1], v1);
+        } else {
+          mfma_v(s[0], f[0], kf[0][kk]);
+          mfma_v(dp[0], f[1], v0);
+          mfma_v(s[1], f[0], kf[1][kk]);
+          mfma_v(dp[1], f[1], v1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      mfma_v_done(s[0], dp[0], s[1], dp[1]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float4 ls = *reinterpret_cast<const float4*>(Lt + 32 * u + 8 * (e >> 2) + 4 * hh);
+          const float4 de = *reinterpret_cast<const float4*>(Dt + 32 * u + 8 * (e >> 2) + 4 * hh);
+          const float l4[4] = {ls.x, ls.y, ls.z, ls.w}, d4[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            s[j][e + x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][e + x], c, -l4[x]));
+            dp[j][e + x] = s[j][e + x] * (dp[j][e + x] - d4[x]);
+          }
+        }
+      if (part) {
+        asm volatile("" ::: "memory");   // a real branch
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const bool seen = (uint32_t)(qsu + 4 * hh - key[j] + crow(e, 0)) < (uint32_t)cnt[j];
+            s[j][e] = seen ? s[j][e] : 0.f;
+            dp[j][e] = seen ? dp[j][e] : 0.f;
+          }
+#pragma unroll
+        for (int kk = 0; kk < NKK; ++kk) bad |= nonfinite(rread(Qu, kk)) | nonfinite(rread(Ou, kk));
+      }
+      bf16x8 pb[2][2], sb[2][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          pb[j][h] = pack8(s[j], 8 * h);
+          sb[j][h] = pack8(dp[j], 8 * h);
+        }
+bf16x8 tf[2][2] = {{tread(Ou, 0), tread(Qu, 0)}, {}};
+#pragma unroll
+      for (int x = 0; x < 2 * NDT; ++x) {             // (16-row half h, 32 columns dt)
+        const int h = x / NDT, dt = x % NDT;
+        bf16x8 (&f)[2] = tf[x & 1], (&n)[2] = tf[(x & 1) ^ 1];
+        if (x + 1 < 2 * NDT) {
+          const int ro = 16 * ((x + 1) / NDT) * RB;
+          n[0] = tread(Ou + ro, (x + 1) % NDT);
+          n[1] = tread(Qu + ro, (x + 1) % NDT);
+        }
+        dvacc[0][dt] = mfma32(f[0], pb[0][h], dvacc[0][dt]);
+        dkacc[0][dt] = mfma32(f[1], sb[0][h], dkacc[0][dt]);
+        dvacc[1][dt] = mfma32(f[0], pb[1][h], dvacc[1][dt]);
+        dkacc[1][dt] = mfma32(f[1], sb[1][h], dkacc[1][dt]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  int hq_n = hk * grp + t0 / nqt, qs_n = k0 + (t0 % nqt) * QT;   // the item to fetch next
+  int qs_c = qs_n;
+  auto advance = [&]() __attribute__((always_inline)) {
+    qs_n += QT;
+    if (qs_n >= qend) { qs_n = k0; ++hq_n; }
+  };
+  issue(ring[0], ring[0] + TILE, stat[0][0], stat[0][1], hq_n, qs_n);
+  advance();
+#pragma unroll 1
+  for (int t = t0; t < t1; ++t) {
+    const int slot = (t - t0) & 1, nslot = slot ^ 1;
+    vm_drain();
+    __syncthreads();
+    const int qs = qs_c;
+    if (t + 1 < t1) {
+      issue(ring[nslot], ring[nslot] + TILE, stat[nslot][0], stat[nslot][1], hq_n, qs_n);
+      qs_c = qs_n;
+      advance();
+    }
+    if (uni(wave_on && qs < emax && qs + QT > kw ? 1 : 0))
+      body(ring[slot], ring[slot] + TILE, stat[slot][0], stat[slot][1], qs);
+  }
+  const int W = a.Hkv * D;
+  float* pk = a.part + (size_t)sp * 2 * T * W + hk * D;   // [split][dk, dv][T][Hkv D]
+  float* pv = pk + (size_t)T * W;
+  if (__any(bad != 0)) {
+#pragma unroll 1
+    for (int j = kw; j <= klast; ++j) {
+      const RowVec<D> kj(a.k + (size_t)j * a.ldk + hk * D, lane);
+      const RowVec<D> vj(a.v + (size_t)j * a.ldv + hk * D, lane);
+      RowVec<D> rk, rv;
+      const int je = a.end[j];
+#pragma unroll 1
+      for (int t = t0; t < t1; ++t) {
+        const int hq = hk * grp + t / nqt, qs = k0 + (t % nqt) * QT;
+#pragma unroll 1
+        for (int i = max(j, qs); i < min(je, qs + QT); ++i) {
+          const RowVec<D> qi(a.q + (size_t)i * a.ldq + hq * D, lane);
+          const RowVec<D> doi(a.dout + (size_t)i * a.lddo + hq * D, lane);
+          const size_t li = (size_t)hq * T + i;
+          const float pij = __builtin_amdgcn_exp2f(__builtin_fmaf(qi.dot(kj), c, -a.lse[li]));
+          rv.axpy(pij, doi);
+          rk.axpy(pij * (doi.dot(vj) - a.delta[li]), qi);
+        }
+      }
+      if (nsp > 1) {
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) {
+          pk[(size_t)j * W + lane + 64 * x] = rk.x[x];
+          pv[(size_t)j * W + lane + 64 * x] = rv.x[x];
+        }
+      } else {
+        rk.store(a.dk + (size_t)j * a.lddk + hk * D, lane, a.scale);
+        rv.store(a.dv + (size_t)j * a.lddv + hk * D, lane, 1.f);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint16_t* dkp = a.dk + (size_t)key[j] * a.lddk + hk * D;
+    uint16_t* dvp = a.dv + (size_t)key[j] * a.lddv + hk * D;
+    if (key[j] >= nv) {
+      if (a.fill && sp == 0 && key[j] < T) {
+        zero_row<D>(dkp, hh);
+        zero_row<D>(dvp, hh);
+      }
+      continue;
+    }
+    if (__any(bad != 0)) continue;
+    if (nsp > 1) {
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const size_t o = (size_t)key[j] * W + 32 * dt + 2 * e + 4 * hh;
+          *reinterpret_cast<float4*>(pk + o) =
+              make_float4(dkacc[j][dt][e], dkacc[j][dt][e + 1], dkacc[j][dt][e + 2], dkacc[j][dt][e + 3]);
+          *reinterpret_cast<float4*>(pv + o) =
+              make_float4(dvacc[j][dt][e], dvacc[j][dt][e + 1], dvacc[j][dt][e + 2], dvacc[j][dt][e + 3]);
+        }
+    } else {
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) {
+        store_row32(dkp + 32 * dt, dkacc[j][dt], a.scale, hh);
+        store_row32(dvp + 32 * dt, dvacc[j][dt], 1.f, hh);
+      }
+    }
+  }
+}
+
+// the partial dK / dV of split blocks, in the order of the splits; 4 values per thread
+template <int D>
+__global__ __launch_bounds__(256) void packed_join_kernel(const PArgs a) {
+  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int W = a.Hkv * D, nw = W / 4;
+  const int64_t t = v / nw;
+  const int nv = a.meta[0];
+  if (t >= nv) return;
+  const int col = (int)(v - t * nw) * 4, k0 = (int)t / KB2 * KB2;
+  const int nqt = (a.end[min(k0 + KB2, nv) - 1] - k0 + QT2 - 1) / QT2;
+  const int nsp = block_splits(nqt * (a.Hq / a.Hkv), a.nsplit);
+  if (nsp == 1) return;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < nsp; ++k) {
+      const float4 x = *reinterpret_cast<const float4*>(a.part + ((size_t)(2 * k + w) * a.T + t) * W + col);
+      s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+    }
+    const float sc = w ? 1.f : a.scale;
+    uint16_t* o = w ? a.dv + (size_t)t * a.lddv : a.dk + (size_t)t * a.lddk;
+    *reinterpret_cast<uint2*>(o + col) = make_uint2(pack2(s.x * sc, s.y * sc), pack2(s.z * sc, s.w * sc));
+  }
+}
+
+// splits of the D = 128 key blocks: enough workgroups for four rounds of the 256 CUs
+int key_splits(int T, int Hkv) {
+  const int64_t blocks = (int64_t)((T + KB2 - 1) / KB2) * Hkv;
+  int n = 1;
+  while (n < 4 && blocks * n < 1024) n *= 2;
+  return n;
+}
+
 bool bad_mat(const void* p, int ld, int width) {   // 16-B rows, tile offsets below 2^31 bytes
   return p == nullptr || ((uintptr_t)p & 15) || (ld & 7) || ld < width || ld > (1 << 22);
 }
@@ -655,12 +987,19 @@ MX_EXPORT int mx_packed_attn_fwd(const void* q, const void* k, const void* v, in
   return hipGetLastError();
 }
 
+// fp32 workspace of mx_packed_attn_bwd beside delta (0: none)
+MX_EXPORT int64_t mx_packed_attn_bwd_floats(int T, int Hkv, int D) {
+  if (T <= 0 || Hkv <= 0 || D != 128) return 0;
+  const int n = key_splits(T, Hkv);
+  return n > 1 ? (int64_t)n * 2 * T * Hkv * D : 0;
+}
+
 // delta: fp32 [Hq][T] workspace (written by the dQ kernel, read by the dK / dV kernel).
 MX_EXPORT int mx_packed_attn_bwd(const void* q, const void* k, const void* v, int ldq, int ldk, int ldv,
                                  const void* o, int ldo, const void* dout, int lddo, const float* lse, float* delta,
                                  void* dq, int lddq, void* dk, void* dv, int lddk, int lddv, const int* start,
                                  const int* end, const int* meta, int T, int Hq, int Hkv, int D, float scale,
-                                 int fill, hipStream_t s) {
+                                 int fill, float* part, int64_t part_floats, hipStream_t s) {
   if (bad_shape(T, Hq, Hkv, D) || bad_mat(q, ldq, Hq * D) || bad_mat(k, ldk, Hkv * D) || bad_mat(v, ldv, Hkv * D) ||
       bad_mat(o, ldo, Hq * D) || bad_mat(dout, lddo, Hq * D) || bad_mat(dq, lddq, Hq * D) ||
       bad_mat(dk, lddk, Hkv * D) || bad_mat(dv, lddv, Hkv * D) || !lse || !delta || !start || !end || !meta ||
@@ -678,13 +1017,22 @@ MX_EXPORT int mx_packed_attn_bwd(const void* q, const void* k, const void* v, in
   a.c = scale * 1.4426950408889634f;
   a.scale = scale;
   a.fill = fill;
+  a.nsplit = D == 128 ? key_splits(T, Hkv) : 1;
+  a.part = part;
+  if (a.nsplit > 1 && (!part || ((uintptr_t)part & 15) || part_floats < mx_packed_attn_bwd_floats(T, Hkv, D)))
+    return hipErrorInvalidValue;
   const unsigned nb = (unsigned)((T + 127) / 128);
   if (D == 64) {
     hipLaunchKernelGGL((packed_qmajor_kernel<64, true>), dim3(nb * Hq), dim3(256), 0, s, a);
     hipLaunchKernelGGL((packed_kmajor_kernel<64>), dim3(nb * Hkv), dim3(256), 0, s, a);
   } else {
     hipLaunchKernelGGL((packed_qmajor_kernel<128, true>), dim3(nb * Hq), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((packed_kmajor_kernel<128>), dim3(nb * Hkv), dim3(256), 0, s, a);
+    const unsigned nk = (unsigned)((T + KB2 - 1) / KB2);
+    hipLaunchKernelGGL((packed_kmajor2_kernel<128>), dim3(nk * Hkv * a.nsplit), dim3(256), 0, s, a);
+    if (a.nsplit > 1) {
+      const int64_t vecs = (int64_t)T * Hkv * 32;
+      hipLaunchKernelGGL((packed_join_kernel<128>), dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, s, a);
+    }
   }
   return hipGetLastError();
 }
