@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void packed_plan_kernel(const IT* __restrict__
 struct PArgs {
   const uint16_t *q, *k, *v, *dout, *o;
   uint16_t *out, *dk, *dv;      // forward: O; backward: dQ, dK, dV
-  float *lse, *delta;           // [Hq][T]
+  float *lse, *nlse, *delta;    // [Hq][T]: log-sum-exp; backward: -lse / c and -delta
   const int *start, *end, *meta;
   int ldq, ldk, ldv, lddo, ldo, ldout, lddk, lddv;
   int T, Hq, Hkv;
@@ -188,7 +188,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
       dl = xhalf_sum(s);
       lse2 = a.lse[(size_t)hq * T + qrow_c];
-      if (hh == 0 && qrow < nv) a.delta[(size_t)hq * T + qrow] = dl;   // read by the dK / dV kernel
+      if (hh == 0 && qrow < nv) {   // what the dK / dV kernel starts its products from
+        a.delta[(size_t)hq * T + qrow] = -dl;
+        a.nlse[(size_t)hq * T + qrow] = -lse2 / a.c;
+      }
     }
   }
   float m_i = -INFINITY, l_i = 0.f;
@@ -492,7 +495,7 @@ packed_kmajor_kernel(const PArgs a) {
     }
     if (wl < 2) {
       const size_t li = (size_t)hq * T + min(qs + lane, nv - 1);
-      if (wl == 0) dma4(a.lse + li, (char*)ld);
+      if (wl == 0) dma4(a.nlse + li, (char*)ld);
       else dma4(a.delta + li, (char*)dd);
     }
   };
@@ -503,7 +506,15 @@ packed_kmajor_kernel(const PArgs a) {
     for (int u = 0; u < NQS; ++u) {
       const int qsu = qs + 32 * u;
       if (uni(qsu + 31 < kw || qsu >= emax ? 1 : 0)) continue;
-      f32x16 s = f32x16{}, dp = f32x16{};
+      // the products start from -lse / c and -delta of their rows: P = 2^(c S), dS = P dP
+      f32x16 s, dp;
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const float4 ls = *reinterpret_cast<const float4*>(Lt + 32 * u + 2 * e + 4 * hh);
+        const float4 de = *reinterpret_cast<const float4*>(Dt + 32 * u + 2 * e + 4 * hh);
+        s[e] = ls.x; s[e + 1] = ls.y; s[e + 2] = ls.z; s[e + 3] = ls.w;
+        dp[e] = de.x; dp[e + 1] = de.y; dp[e + 2] = de.z; dp[e + 3] = de.w;
+      }
       const char* Qu = Qt + 32 * u * RB;
       const char* Ou = Ot + 32 * u * RB;
 #pragma unroll
@@ -512,17 +523,9 @@ packed_kmajor_kernel(const PArgs a) {
         dp = mfma32(lds8(Ou, offQ[kk]), vf[kk], dp);
       }
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const float4 ls = *reinterpret_cast<const float4*>(Lt + 32 * u + 8 * (e >> 2) + 4 * hh);
-        const float4 de = *reinterpret_cast<const float4*>(Dt + 32 * u + 8 * (e >> 2) + 4 * hh);
-        s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -ls.x));
-        s[e + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], c, -ls.y));
-        s[e + 2] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 2], c, -ls.z));
-        s[e + 3] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 3], c, -ls.w));
-        dp[e] = s[e] * (dp[e] - de.x);
-        dp[e + 1] = s[e + 1] * (dp[e + 1] - de.y);
-        dp[e + 2] = s[e + 2] * (dp[e + 2] - de.z);
-        dp[e + 3] = s[e + 3] * (dp[e + 3] - de.w);
+      for (int e = 0; e < 16; ++e) {
+        s[e] = __builtin_amdgcn_exp2f(s[e] * c);
+        dp[e] *= s[e];
       }
       // whole: every row of the subtile sees every key of the wave
       if (uni(qsu < kw + 31 || qsu + 32 > emin || kw + 31 >= nv ? 1 : 0)) {
@@ -593,7 +596,7 @@ packed_kmajor_kernel(const PArgs a) {
           const size_t li = (size_t)hq * T + i;
           const float pij = __builtin_amdgcn_exp2f(__builtin_fmaf(qi.dot(kj), c, -a.lse[li]));
           rv.axpy(pij, doi);
-          rk.axpy(pij * (doi.dot(vj) - a.delta[li]), qi);
+          rk.axpy(pij * (doi.dot(vj) + a.delta[li]), qi);
         }
       rk.store(a.dk + (size_t)j * a.lddk + hk * D, lane, a.scale);
       rv.store(a.dv + (size_t)j * a.lddv + hk * D, lane, 1.f);
@@ -622,24 +625,21 @@ __device__ __forceinline__ int block_splits(int items, int nsplit) { return max(
 // it moved S and dP in and out of them at every subtile.  Written as asm, so the wait between the
 // last product and the first use is mfma_v_done's: 8 passes of 4 cycles and 3 more are required,
 // 24 are waited.  A product's operands are read from LDS (waited for by the compiler) or long loaded.
-__device__ __forceinline__ void mfma_v_first(f32x16& d, bf16x8 a, bf16x8 b) {
-  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
-}
 __device__ __forceinline__ void mfma_v(f32x16& d, bf16x8 a, bf16x8 b) {
   asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
 }
-__device__ __forceinline__ void mfma_v_done(f32x16& a, f32x16& b, f32x16& c, f32x16& d) {
-  asm volatile("s_nop 15\n\ts_nop 7" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+__device__ __forceinline__ void mfma_v_done(f32x16& a, f32x16& b) {
+  asm volatile("s_nop 15\n\ts_nop 7" : "+v"(a), "+v"(b));
 }
 
 template <int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void packed_kmajor2_kernel(const PArgs a) {
-  constexpr int NL = 2;   // V fragments kept in LDS: those the registers do not hold
+  constexpr int NL = 4;   // the V fragments of odd kk stay in LDS: the registers do not hold all
   constexpr int QT = QT2, NQS = QT / 32, NKK = D / 16, NDT = D / 32;
   constexpr int RB = D * 2, CPR = D / 8, RPP = 64 / CPR, TILE = QT * RB, PPW = TILE / 1024 / 4;
   __shared__ __attribute__((aligned(16))) char ring[2][2 * TILE];   // Q, dO
-  __shared__ __attribute__((aligned(16))) float stat[2][2][64];     // lse, delta
-  __shared__ __attribute__((aligned(16))) uint4 vlds[4][2 * NL][64];  // the waves' V fragments of kk < NL
+  __shared__ __attribute__((aligned(16))) float stat[2][2][64];     // -lse / c, -delta
+  __shared__ __attribute__((aligned(16))) uint4 vlds[4][2 * NL][64];  // the waves' V fragments of odd kk
   const int tid = threadIdx.x, lane = tid & 63, wl = uni(tid >> 6);
   const int r = lane & 31, hh = lane >> 5, g = lane >> 4, gi = lane & 15;
   const int T = a.T, nv = uni(a.meta[0]);
@@ -665,7 +665,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   const int klast = min(kw + 63, nv - 1);
   const int emax = uni(a.end[max(klast, 0)]);
   int key[2], cnt[2], emin[2];
-  bf16x8 kf[2][NKK], vf[2][NKK - NL];
+  uint32_t bad = 0;   // (see packed_qmajor_kernel)
+  bf16x8 kf[2][NKK], vf[2][NL];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     key[j] = kw + 32 * j + r;
@@ -677,8 +678,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 #pragma unroll
     for (int kk = 0; kk < NKK; ++kk) {
       kf[j][kk] = ld8(kp + 16 * kk);
-      if (kk < NL) vlds[wl][2 * kk + j][lane] = *reinterpret_cast<const uint4*>(vp + 16 * kk);
-      else vf[j][kk < NL ? 0 : kk - NL] = ld8(vp + 16 * kk);
+      const bf16x8 x = ld8(vp + 16 * kk);
+      bad |= nonfinite(x);
+      if (kk & 1) vlds[wl][kk - 1 + j][lane] = __builtin_bit_cast(uint4, x);
+      else vf[j][kk >> 1] = x;
     }
   }
   f32x16 dvacc[2][NDT], dkacc[2][NDT];
@@ -714,12 +717,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     }
     if (wl < 2) {
       const size_t li = (size_t)hq * T + min(qs + lane, nv - 1);
-      if (wl == 0) dma4(a.lse + li, (char*)ld);
+      if (wl == 0) dma4(a.nlse + li, (char*)ld);
       else dma4(a.delta + li, (char*)dd);
     }
   };
   const float c = a.c;
-  uint32_t bad = 0;   // (see packed_qmajor_kernel)
   auto body = [&](const char* Qt, const char* Ot, const float* Lt, const float* Dt, int qs) __attribute__((always_inline)) {
 #pragma unroll 1
     for (int u = 0; u < NQS; ++u) {
@@ -729,88 +731,118 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       f32x16 s[2], dp[2];
       const char* Qu = Qt + 32 * u * RB;
       const char* Ou = Ot + 32 * u * RB;
+      const float* Lu = Lt + 32 * u + 4 * hh;
+      const float* Du = Dt + 32 * u + 4 * hh;
       // part: some (row, key) pair of the subtile is masked
       const bool part = uni(qsu < kw + 63 || qsu + 32 > emin[0] || qsu + 32 > emin[1] || kw + 63 >= nv ? 1 : 0);
-      // one step's fragments are read under the step before; the barriers keep the compiler from reading
-      // all of them first (there are no registers left for that)
-      auto vread = [&](int x) __attribute__((always_inline)) { return __builtin_bit_cast(bf16x8, vlds[wl][x][lane]); };
-      bf16x8 fr[2][2] = {{rread(Qu, 0), rread(Ou, 0)}, {}};
-      bf16x8 vl[2][2] = {{vread(0), vread(1)}, {}};
-#pragma unroll
-      for (int kk = 0; kk < NKK; ++kk) {
-        bf16x8 (&f)[2] = fr[kk & 1], (&n)[2] = fr[(kk & 1) ^ 1];
-        if (kk + 1 < NKK) {
-          n[0] = rread(Qu, kk + 1);
-          n[1] = rread(Ou, kk + 1);
-        }
-        if (kk + 1 < NL) {
-          vl[(kk & 1) ^ 1][0] = vread(2 * kk + 2);
-          vl[(kk & 1) ^ 1][1] = vread(2 * kk + 3);
-        }
-        const bf16x8 v0 = kk < NL ? vl[kk & 1][0] : vf[0][kk < NL ? 0 : kk - NL];
-        const bf16x8 v1 = kk < NL ? vl[kk & 1][1] : vf[1][kk < NL ? 0 : kk - NL];
-        if (kk == 0) {
-          mfma_v_first(s[0], f[0], kf[0][kk]);
-          mfma_v_first(dp[0], f[1], v0);
-          mfma_v_first(s[1], f[0], kf[1][kk]);
-          mfma_v_first(dp[1], f[1], v1);
-        } else {
-          mfma_v(s[0], f[0], kf[0][kk]);
-          mfma_v(dp[0], f[1], v0);
-          mfma_v(s[1], f[0], kf[1][kk]);
-          mfma_v(dp[1], f[1], v1);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      mfma_v_done(s[0], dp[0], s[1], dp[1]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
+      // One wave per SIMD: vector work runs beside the matrix pipe only where it stands between matrix
+      // instructions.  Four phases of 16 products each -- S; dP between the exponentials; dV between the
+      // products P (dP - delta); dK -- over one stream of 32 LDS fragments, read PD steps (of two products,
+      // 64 cycles) ahead.  The scheduling barriers keep this order (the compiler would read every fragment
+      // first, for which there are no registers).
+      constexpr int PD = 2, RN = PD + 1;
+      bf16x8 f[RN];
+      auto fetch = [&](int x) __attribute__((always_inline)) {
+        if (x < 8) f[x % RN] = rread(Qu, x);
+        else if (x < 16) f[x % RN] = rread(Ou, x - 8);
+        else if (x < 24) f[x % RN] = tread(Ou + 16 * ((x - 16) / NDT) * RB, x % NDT);
+        else if (x < 32) f[x % RN] = tread(Qu + 16 * ((x - 24) / NDT) * RB, x % NDT);
+      };
+      // the products start from -lse / c and -delta of their rows: P = 2^(c S), dS = P dP
+      auto start = [&](f32x16& d, const float* p) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-          const float4 ls = *reinterpret_cast<const float4*>(Lt + 32 * u + 8 * (e >> 2) + 4 * hh);
-          const float4 de = *reinterpret_cast<const float4*>(Dt + 32 * u + 8 * (e >> 2) + 4 * hh);
-          const float l4[4] = {ls.x, ls.y, ls.z, ls.w}, d4[4] = {de.x, de.y, de.z, de.w};
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            s[j][e + x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][e + x], c, -l4[x]));
-            dp[j][e + x] = s[j][e + x] * (dp[j][e + x] - d4[x]);
-          }
+          const float4 x = *reinterpret_cast<const float4*>(p + 2 * e);
+          d[e] = x.x; d[e + 1] = x.y; d[e + 2] = x.z; d[e + 3] = x.w;
         }
+      };
+      start(s[0], Lu);
+      start(s[1], Lu);
+#pragma unroll
+      for (int x = 0; x < PD; ++x) fetch(x);
+      start(dp[0], Du);
+      start(dp[1], Du);
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk) {
+        fetch(kk + PD);
+        mfma_v(s[0], f[kk % RN], kf[0][kk]);
+        mfma_v(s[1], f[kk % RN], kf[1][kk]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      auto vread = [&](int x) __attribute__((always_inline)) { return __builtin_bit_cast(bf16x8, vlds[wl][x][lane]); };
+      bf16x8 vl[2] = {vread(0), vread(1)};
+      auto expo = [&](int x) __attribute__((always_inline)) {   // elements 2 x, 2 x + 1 of both groups: S -> P
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          s[j][2 * x] = __builtin_amdgcn_exp2f(s[j][2 * x] * c);
+          s[j][2 * x + 1] = __builtin_amdgcn_exp2f(s[j][2 * x + 1] * c);
+        }
+      };
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk) {
+        fetch(8 + kk + PD);
+        const bf16x8 v0 = kk & 1 ? vl[0] : vf[0][kk >> 1], v1 = kk & 1 ? vl[1] : vf[1][kk >> 1];
+        mfma_v(dp[0], f[(8 + kk) % RN], v0);
+        mfma_v(dp[1], f[(8 + kk) % RN], v1);
+        if (kk == 0) mfma_v_done(s[0], s[1]);
+        if ((kk & 1) && kk + 2 < NKK) {
+          vl[0] = vread(kk + 1);
+          vl[1] = vread(kk + 2);
+        }
+        expo(kk);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      static_assert(NKK == 8 && NDT == 4, "the phases carry 16 elements in 8 steps");
+      auto grad = [&](int x) __attribute__((always_inline)) {   // elements 2 x, 2 x + 1: dP -> dS
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          dp[j][2 * x] *= s[j][2 * x];
+          dp[j][2 * x + 1] *= s[j][2 * x + 1];
+        }
+      };
       if (part) {
+        // P = 0 where masked; dS = P (dP - delta) is then 0 too unless a factor is not finite, which marks
+        // the wave (dO, Q and delta here; its V rows were looked at when they were loaded)
         asm volatile("" ::: "memory");   // a real branch
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const bool seen = (uint32_t)(qsu + 4 * hh - key[j] + crow(e, 0)) < (uint32_t)cnt[j];
-            s[j][e] = seen ? s[j][e] : 0.f;
-            dp[j][e] = seen ? dp[j][e] : 0.f;
-          }
+          for (int e = 0; e < 16; ++e)
+            s[j][e] = (uint32_t)(qsu + 4 * hh - key[j] + crow(e, 0)) < (uint32_t)cnt[j] ? s[j][e] : 0.f;
 #pragma unroll
         for (int kk = 0; kk < NKK; ++kk) bad |= nonfinite(rread(Qu, kk)) | nonfinite(rread(Ou, kk));
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const float2 de = *reinterpret_cast<const float2*>(Du + 8 * (x >> 1) + 2 * (x & 1));
+          bad |= !(fabsf(de.x) < INFINITY) || !(fabsf(de.y) < INFINITY) ? 0x8000u : 0u;
+        }
       }
-      bf16x8 pb[2][2], sb[2][2];
+      bf16x8 w[2][2];                                  // P, then dS, of both groups as MFMA operands
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          pb[j][h] = pack8(s[j], 8 * h);
-          sb[j][h] = pack8(dp[j], 8 * h);
-        }
-bf16x8 tf[2][2] = {{tread(Ou, 0), tread(Qu, 0)}, {}};
+        for (int h = 0; h < 2; ++h) w[j][h] = pack8(s[j], 8 * h);
+      auto dv_step = [&](int x) __attribute__((always_inline)) {   // (16-row half x / 4, 32 columns x % 4)
+        fetch(16 + x + PD);
+        dvacc[0][x % NDT] = mfma32(f[(16 + x) % RN], w[0][x / NDT], dvacc[0][x % NDT]);
+        dvacc[1][x % NDT] = mfma32(f[(16 + x) % RN], w[1][x / NDT], dvacc[1][x % NDT]);
+      };
 #pragma unroll
-      for (int x = 0; x < 2 * NDT; ++x) {             // (16-row half h, 32 columns dt)
-        const int h = x / NDT, dt = x % NDT;
-        bf16x8 (&f)[2] = tf[x & 1], (&n)[2] = tf[(x & 1) ^ 1];
-        if (x + 1 < 2 * NDT) {
-          const int ro = 16 * ((x + 1) / NDT) * RB;
-          n[0] = tread(Ou + ro, (x + 1) % NDT);
-          n[1] = tread(Qu + ro, (x + 1) % NDT);
-        }
-        dvacc[0][dt] = mfma32(f[0], pb[0][h], dvacc[0][dt]);
-        dkacc[0][dt] = mfma32(f[1], sb[0][h], dkacc[0][dt]);
-        dvacc[1][dt] = mfma32(f[0], pb[1][h], dvacc[1][dt]);
-        dkacc[1][dt] = mfma32(f[1], sb[1][h], dkacc[1][dt]);
+      for (int x = 0; x < 8; ++x) {
+        dv_step(x);
+        if (x == 0) mfma_v_done(dp[0], dp[1]);
+        grad(x);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[j][h] = pack8(dp[j], 8 * h);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        fetch(24 + x + PD);
+        dkacc[0][x % NDT] = mfma32(f[(24 + x) % RN], w[0][x / NDT], dkacc[0][x % NDT]);
+        dkacc[1][x % NDT] = mfma32(f[(24 + x) % RN], w[1][x / NDT], dkacc[1][x % NDT]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -857,7 +889,7 @@ bf16x8 tf[2][2] = {{tread(Ou, 0), tread(Qu, 0)}, {}};
           const size_t li = (size_t)hq * T + i;
           const float pij = __builtin_amdgcn_exp2f(__builtin_fmaf(qi.dot(kj), c, -a.lse[li]));
           rv.axpy(pij, doi);
-          rk.axpy(pij * (doi.dot(vj) - a.delta[li]), qi);
+          rk.axpy(pij * (doi.dot(vj) + a.delta[li]), qi);
         }
       }
       if (nsp > 1) {
@@ -987,30 +1019,31 @@ MX_EXPORT int mx_packed_attn_fwd(const void* q, const void* k, const void* v, in
   return hipGetLastError();
 }
 
-// fp32 workspace of mx_packed_attn_bwd beside delta (0: none)
+// floats of `part` (0: none)
 MX_EXPORT int64_t mx_packed_attn_bwd_floats(int T, int Hkv, int D) {
   if (T <= 0 || Hkv <= 0 || D != 128) return 0;
   const int n = key_splits(T, Hkv);
   return n > 1 ? (int64_t)n * 2 * T * Hkv * D : 0;
 }
 
-// delta: fp32 [Hq][T] workspace (written by the dQ kernel, read by the dK / dV kernel).
+// stats: fp32 [2][Hq][T] workspace (written by the dQ kernel, read by the dK / dV kernel).
 MX_EXPORT int mx_packed_attn_bwd(const void* q, const void* k, const void* v, int ldq, int ldk, int ldv,
-                                 const void* o, int ldo, const void* dout, int lddo, const float* lse, float* delta,
+                                 const void* o, int ldo, const void* dout, int lddo, const float* lse, float* stats,
                                  void* dq, int lddq, void* dk, void* dv, int lddk, int lddv, const int* start,
                                  const int* end, const int* meta, int T, int Hq, int Hkv, int D, float scale,
                                  int fill, float* part, int64_t part_floats, hipStream_t s) {
   if (bad_shape(T, Hq, Hkv, D) || bad_mat(q, ldq, Hq * D) || bad_mat(k, ldk, Hkv * D) || bad_mat(v, ldv, Hkv * D) ||
       bad_mat(o, ldo, Hq * D) || bad_mat(dout, lddo, Hq * D) || bad_mat(dq, lddq, Hq * D) ||
-      bad_mat(dk, lddk, Hkv * D) || bad_mat(dv, lddv, Hkv * D) || !lse || !delta || !start || !end || !meta ||
-      !(scale > 0.f))
+      bad_mat(dk, lddk, Hkv * D) || bad_mat(dv, lddv, Hkv * D) || !lse || !stats || ((uintptr_t)stats & 3) || !start ||
+      !end || !meta || !(scale > 0.f))
     return hipErrorInvalidValue;
   PArgs a{};
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
   a.o = (const uint16_t*)o; a.dout = (const uint16_t*)dout;
   a.out = (uint16_t*)dq; a.dk = (uint16_t*)dk; a.dv = (uint16_t*)dv;
   a.lse = const_cast<float*>(lse);
-  a.delta = delta;
+  a.nlse = stats;
+  a.delta = stats + (size_t)Hq * T;
   a.start = start; a.end = end; a.meta = meta;
   a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo; a.lddo = lddo; a.ldout = lddq; a.lddk = lddk; a.lddv = lddv;
   a.T = T; a.Hq = Hq; a.Hkv = Hkv;

@@ -206,11 +206,11 @@ def packed_attn_bwd(dout, q, k, v, o, lse, seqs: PackedSequences, Hq: int, Hkv: 
             dq = torch.empty(seqs.total, Hq * D, dtype=q.dtype, device=q.device)
             dk = torch.empty(seqs.total, Hkv * D, dtype=q.dtype, device=q.device)
             dv = torch.empty(seqs.total, Hkv * D, dtype=q.dtype, device=q.device)
-        delta = torch.empty(Hq, seqs.total, dtype=torch.float32, device=q.device)
+        stats = torch.empty(2, Hq, seqs.total, dtype=torch.float32, device=q.device)
         nf = _lib.query64("mx_packed_attn_bwd_floats", seqs.total, Hkv, D)
         part = torch.empty(nf, dtype=torch.float32, device=q.device) if nf else None
         _lib.call("mx_packed_attn_bwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _ld(q), _ld(k), _ld(v),
-                  _lib.ptr(o), _ld(o), _lib.ptr(dout), _ld(dout), _lib.ptr(lse), _lib.ptr(delta),
+                  _lib.ptr(o), _ld(o), _lib.ptr(dout), _ld(dout), _lib.ptr(lse), _lib.ptr(stats),
                   _lib.ptr(dq), _ld(dq), _lib.ptr(dk), _lib.ptr(dv), _ld(dk), _ld(dv),
                   _lib.ptr(seqs.start), _lib.ptr(seqs.end), _lib.ptr(seqs.meta), seqs.total, Hq, Hkv, D, scale,
                   int(not given[0]), _lib.ptr(part), nf, _lib.stream())
