@@ -92,30 +92,11 @@ __device__ __forceinline__ uint64_t match_digit(int d, int bits, uint64_t live) 
   return m;
 }
 
-// Stable scatter of one block's tokens: wave w owns the w-th contiguous share.  wcnt[w][d] counts
-// the share's digits, then holds the next output slot of digit d for that wave.
-__global__ __launch_bounds__(SORT_NT) void sort_scatter_kernel(const SortArgs a) {
-  extern __shared__ int smem[];
-  const int R = 1 << a.bits, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  int* wcnt = smem;                       // [SORT_NW][R]
-  int* tot = smem + SORT_NW * R;          // [R]
-  __shared__ int wsum[SORT_NW];
-  for (int i = tid; i < SORT_NW * R; i += SORT_NT) wcnt[i] = 0;
-  __syncthreads();
-  const int t0 = blockIdx.x * a.tpb, share = a.tpb / SORT_NW;
-  const int s0 = t0 + w * share, s1 = min(a.T, s0 + share);
-  for (int t = s0 + lane; t < s1; t += 64) atomicAdd(&wcnt[w * R + ((sort_key(a, t) >> a.shift) & (R - 1))], 1);
-  __syncthreads();
-  // first slot of (this block, digit): digits below it anywhere, then the blocks before this one
-  int mine = 0, before = 0;               // R <= SORT_NT: one digit per thread
-  if (tid < R) {
-    for (int b = 0; b < (int)gridDim.x; ++b) {
-      const int c = a.hist[b * R + tid];
-      mine += c;
-      before += b < (int)blockIdx.x ? c : 0;
-    }
-  }
-  int x = mine;                           // inclusive scan over the digits: wave, then waves
+// Next output slot of every (wave, digit): wcnt holds the waves' digit counts on entry; `total` and
+// `before` are the digit's count anywhere and in the blocks before this one (digit = threadIdx.x)
+__device__ __forceinline__ void digit_slots(int* wcnt, int* wsum, int R, int total, int before) {
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  int x = total;                          // inclusive scan over the digits: wave, then waves
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int y = __shfl_up(x, o);
@@ -125,10 +106,8 @@ __global__ __launch_bounds__(SORT_NT) void sort_scatter_kernel(const SortArgs a)
   __syncthreads();
   int off = 0;
   for (int i = 0; i < w; ++i) off += wsum[i];
-  if (tid < R) tot[tid] = off + x - mine + before;
-  __syncthreads();
-  if (tid < R) {                          // per-wave start slots
-    int s = tot[tid];
+  if (tid < R) {                          // R <= SORT_NT: one digit per thread
+    int s = off + x - total + before;
     for (int i = 0; i < SORT_NW; ++i) {
       const int c = wcnt[i * R + tid];
       wcnt[i * R + tid] = s;
@@ -136,19 +115,90 @@ __global__ __launch_bounds__(SORT_NT) void sort_scatter_kernel(const SortArgs a)
     }
   }
   __syncthreads();
+}
+// slot of this lane's digit among its wave's tokens, in token order (wcnt: the wave's slots)
+__device__ __forceinline__ int take_slot(int* wcnt, int d, int bits, bool live, int lane) {
+  const uint64_t peers = match_digit(d, bits, __ballot(live));
+  const int rank = __popcll(peers & ((1ull << lane) - 1)), lead = __ffsll((unsigned long long)peers) - 1;
+  int slot = 0;
+  if (live && rank == 0) slot = atomicAdd(&wcnt[d], __popcll(peers));
+  return __shfl(slot, live ? lead : lane) + rank;
+}
+
+// Stable scatter of one block's tokens: wave w owns the w-th contiguous share.
+__global__ __launch_bounds__(SORT_NT) void sort_scatter_kernel(const SortArgs a) {
+  extern __shared__ int wcnt[];           // [SORT_NW][R]
+  __shared__ int wsum[SORT_NW];
+  const int R = 1 << a.bits, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  for (int i = tid; i < SORT_NW * R; i += SORT_NT) wcnt[i] = 0;
+  __syncthreads();
+  const int share = a.tpb / SORT_NW;
+  const int s0 = blockIdx.x * a.tpb + w * share, s1 = min(a.T, s0 + share);
+  for (int t = s0 + lane; t < s1; t += 64) atomicAdd(&wcnt[w * R + ((sort_key(a, t) >> a.shift) & (R - 1))], 1);
+  __syncthreads();
+  int total = 0, before = 0;
+  if (tid < R) {
+#pragma unroll 8
+    for (int b = 0; b < (int)gridDim.x; ++b) {
+      const int c = a.hist[b * R + tid];
+      total += c;
+      before += b < (int)blockIdx.x ? c : 0;
+    }
+  }
+  digit_slots(wcnt, wsum, R, total, before);
   for (int c0 = s0; c0 < s1; c0 += 64) {
     const int t = c0 + lane;
     const bool live = t < s1;
     const int key = live ? sort_key(a, t) : 0, d = (key >> a.shift) & (R - 1);
-    const uint64_t peers = match_digit(d, a.bits, __ballot(live));
-    const int rank = __popcll(peers & ((1ull << lane) - 1)), lead = __ffsll((unsigned long long)peers) - 1;
-    int slot = 0;
-    if (live && rank == 0) slot = atomicAdd(&wcnt[w * R + d], __popcll(peers));
-    slot = __shfl(slot, live ? lead : lane) + rank;
+    const int slot = take_slot(wcnt + w * R, d, a.bits, live, lane);
     if (live) {
       a.kout[slot] = key;
       a.iout[slot] = a.iin ? a.iin[t] : t;
     }
+  }
+}
+
+// The whole sort of up to SMALL tokens in one workgroup and one launch, the pairs in LDS: at 4096
+// tokens two digit passes cost less than the launches of the block form (17 us).
+constexpr int SMALL = 8192;
+__global__ __launch_bounds__(SORT_NT) void sort_small_kernel(const SortArgs a, int passes) {
+  __shared__ int keys[2][SMALL];
+  __shared__ uint16_t idx[2][SMALL];
+  __shared__ int wcnt[SORT_NW << MAX_BITS];
+  __shared__ int wsum[SORT_NW];
+  const int R = 1 << a.bits, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, T = a.T;
+  const int share = ((T + 64 * SORT_NW - 1) / (64 * SORT_NW)) * 64;
+  const int s0 = min(T, w * share), s1 = min(T, s0 + share);
+  for (int t = tid; t < T; t += SORT_NT) {
+    keys[0][t] = sort_key(a, t);
+    idx[0][t] = (uint16_t)t;
+  }
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * a.bits, in = p & 1, out = in ^ 1;
+    for (int i = tid; i < SORT_NW * R; i += SORT_NT) wcnt[i] = 0;
+    __syncthreads();
+    for (int t = s0 + lane; t < s1; t += 64) atomicAdd(&wcnt[w * R + ((keys[in][t] >> shift) & (R - 1))], 1);
+    __syncthreads();
+    int total = 0;
+    if (tid < R)
+      for (int i = 0; i < SORT_NW; ++i) total += wcnt[i * R + tid];
+    digit_slots(wcnt, wsum, R, total, 0);
+    for (int c0 = s0; c0 < s1; c0 += 64) {
+      const int t = c0 + lane;
+      const bool live = t < s1;
+      const int key = live ? keys[in][t] : 0;
+      const int slot = take_slot(wcnt + w * R, (key >> shift) & (R - 1), a.bits, live, lane);
+      if (live) {
+        keys[out][slot] = key;
+        idx[out][slot] = idx[in][t];
+      }
+    }
+    __syncthreads();
+  }
+  const int fin = passes & 1;
+  for (int t = tid; t < T; t += SORT_NT) {
+    a.kout[t] = keys[fin][t];
+    a.iout[t] = idx[fin][t];
   }
 }
 
@@ -329,8 +379,13 @@ MX_EXPORT int mx_embedding_bwd(const void* ids, int64_t vstart, const void* dout
   int *k0 = b, *i0 = b + t4, *k1 = b + 2 * t4, *i1 = b + 3 * t4, *hist = b + 4 * t4;
   float* part = (float*)(hist + (((int64_t)p.blocks << p.bits) + 3 & ~3ll));
   SortArgs a{(const int64_t*)ids, vstart, V, T, p.tpb, nullptr, nullptr, k0, i0, hist, 0, p.bits};
-  const size_t lds = (size_t)(SORT_NW + 1) * sizeof(int) << p.bits;
-  for (int q = 0; q < p.passes; ++q) {
+  if (T <= SMALL) {
+    hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(SORT_NT), 0, s, a, p.passes);
+    a.kin = k0;
+    a.iin = i0;
+  }
+  const size_t lds = (size_t)SORT_NW * sizeof(int) << p.bits;
+  for (int q = 0; q < (T <= SMALL ? 0 : p.passes); ++q) {
     a.shift = q * p.bits;
     hipLaunchKernelGGL(sort_hist_kernel, dim3(p.blocks), dim3(SORT_NT), 0, s, a);
     hipLaunchKernelGGL(sort_scatter_kernel, dim3(p.blocks), dim3(SORT_NT), lds, s, a);

@@ -7,6 +7,7 @@ reference path for debugging).  CPU tensors always use the reference path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -246,6 +247,31 @@ def ptr(t):
     if t is None:
         return None
     return t.data_ptr()
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(t):
+    """Context in which ``t``'s device is the current one (its current stream is then the launch
+    stream); free when it already is."""
+    return _SAME_DEVICE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def rows_of(t, rows, cols, dev, ld_max):
+    """(address, row stride) of a bfloat16 [rows, cols] matrix on device index ``dev`` that the
+    kernels take in place -- unit column stride, 16-byte aligned rows that do not overlap -- or
+    None.  (One pass over the attributes: the checks of a small call would cost more than its
+    kernel; the ops name what is wrong only when this returns None.)"""
+    if t.dtype is not torch.bfloat16 or t.shape != (rows, cols) or t.get_device() != dev:
+        return None
+    p = t.data_ptr()
+    ld, c = t.stride()
+    if rows == 1:       # (a single row has no stride)
+        ld = cols
+    if c != 1 or ld % 8 or not cols <= ld <= ld_max or p % 16:
+        return None
+    return p, ld
 
 
 def _fn(name):

@@ -87,7 +87,7 @@ def embedding_fwd(ids, wte, scale: float = 1.0, positions=None, wpe=None, vocab_
         _check_hip(name, "wpe", wpe, H)
     ids = ids.contiguous()
     pos = positions.contiguous() if positions is not None else None
-    with torch.cuda.device(dev):
+    with _lib.on_device(wte):
         out = torch.empty(T, H, dtype=wte.dtype, device=dev)
         _lib.call("mx_embedding_fwd", _lib.ptr(ids), _lib.ptr(wte), vocab_start, V, scale, _lib.ptr(pos),
                   _lib.ptr(wpe), wpe.shape[0] if wpe is not None else 0, _lib.ptr(out), T, H, _lib.stream())
@@ -132,7 +132,7 @@ def embedding_bwd(keys, dout, rows: int, scale: float = 1.0, out=None, accumulat
     _check_hip(name, "dout", dout[:1], H)
     keys = keys.contiguous()
     ld = dout.stride(0) if T > 1 else H
-    with torch.cuda.device(dev):
+    with _lib.on_device(dout):
         words = _lib.query64("mx_embedding_bwd_words", T, rows, H)
         if words < 0:
             raise ValueError(f"{name}: {T} tokens, {rows} rows are more than the kernels take (2^30)")

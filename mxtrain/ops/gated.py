@@ -84,6 +84,29 @@ def _check(name, act, x, w1, b1, w2, b2, **more):
     return T, H, F, Ho, hip
 
 
+def _mats(act, x, w1, b1, w2, b2):
+    """Sizes, (address, row stride) of x, w1, w2 and the bias addresses of a valid GPU call, or None:
+    a CPU call, no tokens, or a call whose fault :func:`_check` names."""
+    if act not in ACTS or not _lib.use_hip(x) or x.dim() != 2 or w2.dim() != 2:
+        return None
+    (T, H), (Ho, F) = x.shape, w2.shape
+    if (H | F | Ho) % 8 or not 0 < T <= MAX_TOKENS or max(H, 2 * F, Ho) > 1 << 20 or not H or not F or not Ho:
+        return None
+    dev = x.get_device()
+    mats = [_lib.rows_of(t, r, c, dev, 1 << 21) for t, r, c in ((x, T, H), (w1, 2 * F, H), (w2, Ho, F))]
+    if None in mats:
+        return None
+    for b, n in ((b1, 2 * F), (b2, Ho)):
+        p = None
+        if b is not None:
+            p = b.data_ptr()
+            if b.dtype is not torch.bfloat16 or b.shape != (n,) or b.get_device() != dev or not b.is_contiguous() \
+                    or p % 16:
+                return None
+        mats.append(p)
+    return (T, H, F, Ho), *mats
+
+
 # ------------------------------------------------------------------ tiles
 # Per tile of csrc/gated.hip: (rows, columns, workgroups per CU, us per 64-deep step, us per round of
 # workgroups beside the steps), fitted to one MI355X over 4096 x 4096 x 10880 (steps) and
@@ -132,8 +155,11 @@ def _split_ws(splits, M, N, device):
 def gated_mlp_fwd(x, w1, b1, w2, b2, act: str = "silu", save: bool = True):
     """x [T, H] -> (y [T, Ho], pre [T, 2F], h [T, F]); without ``save`` the last two are None.
     Biases may be None."""
-    T, H, F, Ho, hip = _check("gated_mlp_fwd", act, x, w1, b1, w2, b2)
-    if not hip:
+    m = _mats(act, x, w1, b1, w2, b2)
+    if m is None:
+        T, H, F, Ho, hip = _check("gated_mlp_fwd", act, x, w1, b1, w2, b2)
+        if hip and T:
+            raise ValueError("gated_mlp_fwd: unsupported arguments")
         pre = _acc(x) @ _acc(w1).t()
         if b1 is not None:
             pre = pre + _acc(b1)
@@ -143,17 +169,18 @@ def gated_mlp_fwd(x, w1, b1, w2, b2, act: str = "silu", save: bool = True):
             y = y + _acc(b2)
         y = y.to(x.dtype)
         return (y, pre.to(x.dtype), h.to(x.dtype)) if save else (y, None, None)
-    with torch.cuda.device(x.device):
+    (T, H, F, Ho), (x_, ldx), (w1_, ld1), (w2_, ld2), b1_, b2_ = m
+    with _lib.on_device(x):
         y = torch.empty(T, Ho, dtype=x.dtype, device=x.device)
         h = torch.empty(T, F, dtype=x.dtype, device=x.device)
         pre = torch.empty(T, 2 * F, dtype=x.dtype, device=x.device) if save else None
-        if T:
-            _lib.call("mx_gated_fwd", _lib.ptr(x), _ld(x), _lib.ptr(w1), _ld(w1), _lib.ptr(b1), _lib.ptr(pre),
-                      _lib.ptr(h), T, H, F, ACTS[act], _plan("gate", T, 2 * F, H)[0], _lib.stream())
-            tile, splits = _plan("down", T, Ho, F)
-            part = _split_ws(splits, T, Ho, x.device)
-            _lib.call("mx_gated_down", _lib.ptr(h), _lib.ptr(w2), _ld(w2), _lib.ptr(b2), _lib.ptr(y), T, Ho, F,
-                      tile, splits, _lib.ptr(part), _lib.stream())
+        s = _lib.stream()
+        _lib.call("mx_gated_fwd", x_, ldx, w1_, ld1, b1_, _lib.ptr(pre), h.data_ptr(), T, H, F, ACTS[act],
+                  _plan("gate", T, 2 * F, H)[0], s)
+        tile, splits = _plan("down", T, Ho, F)
+        part = _split_ws(splits, T, Ho, x.device)
+        _lib.call("mx_gated_down", h.data_ptr(), w2_, ld2, b2_, y.data_ptr(), T, Ho, F, tile, splits, _lib.ptr(part),
+                  s)
     return (y, pre, h) if save else (y, None, None)
 
 
@@ -203,7 +230,7 @@ def gated_mlp_bwd(dy, x, pre, h, w1, b1, w2, b2, act: str = "silu", dw1=None, db
                 if buf is not None:
                     buf.copy_(_acc(buf) + val if accumulate else val)
         return ((dpre @ _acc(w1)).to(x.dtype) if need_dx else None), dw1, db1, dw2, db2
-    with torch.cuda.device(x.device):
+    with _lib.on_device(x):
         s = _lib.stream()
         dpre = torch.empty(T, 2 * F, dtype=x.dtype, device=x.device)
         part = buf = None

@@ -27,11 +27,12 @@ class PackedSequences:
     the bounds of its sequence (``start``, ``end``, int32) and its position in it
     (``positions``, int64: RoPE's ``pos_ids``, the rows of a learned position table)."""
 
-    __slots__ = ("cu_seqlens", "total", "start", "end", "meta", "positions")
+    __slots__ = ("cu_seqlens", "total", "start", "end", "meta", "positions", "ptrs")
 
     def __init__(self, cu_seqlens, total, start, end, meta, positions):
         self.cu_seqlens, self.total = cu_seqlens, total
         self.start, self.end, self.meta, self.positions = start, end, meta, positions
+        self.ptrs = (start.data_ptr(), end.data_ptr(), meta.data_ptr())   # (this object owns the tensors)
 
     @property
     def device(self):
@@ -67,7 +68,7 @@ def pack_sequences(cu_seqlens: torch.Tensor, total: int, device=None) -> PackedS
         end = torch.where(real, cu.to(torch.int64)[i + 1], t)
         meta = torch.tensor([nv, 0, 0, 0], dtype=torch.int32, device=dev)
         return PackedSequences(cu, total, start.int(), end.int(), meta, t - start)
-    with torch.cuda.device(cu.device):
+    with _lib.on_device(cu):
         tab = torch.empty(2 * total + 4, dtype=torch.int32, device=cu.device)
         pos = torch.empty(total, dtype=torch.int64, device=cu.device)
         start, end, meta = tab[:total], tab[total:2 * total], tab[2 * total:]
@@ -120,10 +121,21 @@ def _readable(t):
             and t.data_ptr() % 16 == 0)
 
 
-def _check_lse(name, lse, Hq, seqs):
-    if tuple(lse.shape) != (Hq, seqs.total) or lse.dtype != torch.float32 or not lse.is_contiguous() \
-            or lse.device != seqs.device:
-        raise ValueError(f"{name}: lse must be the float32 [{Hq}, {seqs.total}] tensor packed_attn_fwd returned")
+def _mats(seqs, Hq, Hkv, D, scale, q, *mats):
+    """[(address, row stride)] of a valid GPU call's matrices (None for those not given), or None: a
+    CPU call, or one whose fault :func:`_check` names."""
+    if (type(seqs) is not PackedSequences or not _lib.use_hip(q) or (D != 64 and D != 128) or Hkv <= 0 or Hq <= 0
+            or Hq % Hkv or not (scale is None or 0.0 < scale < math.inf)):
+        return None
+    dev, T, out = seqs.start.get_device(), seqs.total, []
+    for t, heads in mats:
+        m = None
+        if t is not None:
+            m = _lib.rows_of(t, T, heads * D, dev, 1 << 22)
+            if m is None:
+                return None
+        out.append(m)
+    return out
 
 
 # ------------------------------------------------------------------ reference (CPU)
@@ -169,16 +181,21 @@ def packed_attn_fwd(q, k, v, seqs: PackedSequences, Hq: int, Hkv: int, D: int, s
                     out=None):
     """Causal attention within each sequence: q [T, Hq*D], k / v [T, Hkv*D] -> (o [T, Hq*D],
     lse [Hq, T]).  Query head h reads key head h // (Hq // Hkv).  ``out``: a buffer for o."""
-    scale, hip = _check("packed_attn_fwd", seqs, Hq, Hkv, D, scale, q=q, k=k, v=v, out=out)
-    if not hip:
-        o, lse = _ref_fwd(q, k, v, seqs, Hq, Hkv, D, scale)
-        return _emit(o.to(q.dtype), out, seqs), lse.float()
-    with torch.cuda.device(q.device):
-        o = out if out is not None else torch.empty(seqs.total, Hq * D, dtype=q.dtype, device=q.device)
-        lse = torch.empty(Hq, seqs.total, dtype=torch.float32, device=q.device)
-        _lib.call("mx_packed_attn_fwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _ld(q), _ld(k), _ld(v),
-                  _lib.ptr(o), _ld(o), _lib.ptr(lse), _lib.ptr(seqs.start), _lib.ptr(seqs.end),
-                  _lib.ptr(seqs.meta), seqs.total, Hq, Hkv, D, scale, int(out is None), _lib.stream())
+    m = _mats(seqs, Hq, Hkv, D, scale, q, (q, Hq), (k, Hkv), (v, Hkv), (out, Hq))
+    if m is None:
+        scale, hip = _check("packed_attn_fwd", seqs, Hq, Hkv, D, scale, q=q, k=k, v=v, out=out)
+        if not hip:
+            o, lse = _ref_fwd(q, k, v, seqs, Hq, Hkv, D, scale)
+            return _emit(o.to(q.dtype), out, seqs), lse.float()
+        raise ValueError("packed_attn_fwd: unsupported arguments")
+    T = seqs.total
+    (q_, ldq), (k_, ldk), (v_, ldv), o_ = m
+    with _lib.on_device(q):
+        o = out if out is not None else torch.empty(T, Hq * D, dtype=q.dtype, device=q.device)
+        lse = torch.empty(Hq, T, dtype=torch.float32, device=q.device)
+        _lib.call("mx_packed_attn_fwd", q_, k_, v_, ldq, ldk, ldv, o.data_ptr(), o_[1] if o_ else Hq * D,
+                  lse.data_ptr(), *seqs.ptrs, T, Hq, Hkv, D, D ** -0.5 if scale is None else scale, int(out is None),
+                  _lib.stream())
     return o, lse
 
 
@@ -186,34 +203,42 @@ def packed_attn_bwd(dout, q, k, v, o, lse, seqs: PackedSequences, Hq: int, Hkv: 
                     scale: Optional[float] = None, dq=None, dk=None, dv=None):
     """(dq, dk, dv) of :func:`packed_attn_fwd`; given views (e.g. column ranges of one packed
     dqkv) are written in place.  Deterministic: no atomics."""
-    scale, hip = _check("packed_attn_bwd", seqs, Hq, Hkv, D, scale, q=q, k=k, v=v, dout=dout, o=o, dq=dq, dk=dk,
-                        dv=dv)
-    _check_lse("packed_attn_bwd", lse, Hq, seqs)
-    if not hip:
+    m = _mats(seqs, Hq, Hkv, D, scale, q, (q, Hq), (k, Hkv), (v, Hkv), (o, Hq), (dout, Hq), (dq, Hq), (dk, Hkv),
+              (dv, Hkv))
+    if m is None:
+        scale, hip = _check("packed_attn_bwd", seqs, Hq, Hkv, D, scale, q=q, k=k, v=v, dout=dout, o=o, dq=dq, dk=dk,
+                            dv=dv)
+        if hip:
+            raise ValueError("packed_attn_bwd: unsupported arguments")
+    if lse.shape != (Hq, seqs.total) or lse.dtype is not torch.float32 or not lse.is_contiguous() \
+            or lse.device != q.device:
+        raise ValueError(f"packed_attn_bwd: lse must be the float32 [{Hq}, {seqs.total}] tensor packed_attn_fwd returned")
+    if m is None:
         with torch.enable_grad():
             leaves = [_acc(t.detach()).clone().requires_grad_(True) for t in (q, k, v)]
             of, _ = _ref_fwd(*leaves, seqs, Hq, Hkv, D, scale)
             nv = int(seqs.meta[0])
             grads = torch.autograd.grad(of[:nv], leaves, _acc(dout)[:nv])
         return tuple(_emit(g.to(q.dtype), buf, seqs) for g, buf in zip(grads, (dq, dk, dv)))
-    given = [t is not None for t in (dq, dk, dv)]
-    if any(given) and not all(given):
+    T, given = seqs.total, dq is not None
+    if (dk is not None) != given or (dv is not None) != given:
         raise ValueError("packed_attn_bwd: give all of dq, dk, dv or none")
-    if given[0] and {t.data_ptr() for t in (dq, dk, dv)} & {t.data_ptr() for t in (q, k, v, o, dout)}:
+    (q_, ldq), (k_, ldk), (v_, ldv), (o_, ldo), (do_, lddo), *grads = m
+    if given and {g[0] for g in grads} & {q_, k_, v_, o_, do_}:
         raise ValueError("packed_attn_bwd: dq, dk, dv must not lie over q, k, v, o or dout (read after they are written)")
-    with torch.cuda.device(q.device):
-        if dq is None:
-            dq = torch.empty(seqs.total, Hq * D, dtype=q.dtype, device=q.device)
-            dk = torch.empty(seqs.total, Hkv * D, dtype=q.dtype, device=q.device)
-            dv = torch.empty(seqs.total, Hkv * D, dtype=q.dtype, device=q.device)
-        stats = torch.empty(2, Hq, seqs.total, dtype=torch.float32, device=q.device)
-        nf = _lib.query64("mx_packed_attn_bwd_floats", seqs.total, Hkv, D)
+    with _lib.on_device(q):
+        if not given:
+            dq = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device)
+            dk = torch.empty(T, Hkv * D, dtype=q.dtype, device=q.device)
+            dv = torch.empty(T, Hkv * D, dtype=q.dtype, device=q.device)
+            grads = (dq.data_ptr(), Hq * D), (dk.data_ptr(), Hkv * D), (dv.data_ptr(), Hkv * D)
+        stats = torch.empty(2, Hq, T, dtype=torch.float32, device=q.device)
+        nf = _lib.query64("mx_packed_attn_bwd_floats", T, Hkv, D)
         part = torch.empty(nf, dtype=torch.float32, device=q.device) if nf else None
-        _lib.call("mx_packed_attn_bwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _ld(q), _ld(k), _ld(v),
-                  _lib.ptr(o), _ld(o), _lib.ptr(dout), _ld(dout), _lib.ptr(lse), _lib.ptr(stats),
-                  _lib.ptr(dq), _ld(dq), _lib.ptr(dk), _lib.ptr(dv), _ld(dk), _ld(dv),
-                  _lib.ptr(seqs.start), _lib.ptr(seqs.end), _lib.ptr(seqs.meta), seqs.total, Hq, Hkv, D, scale,
-                  int(not given[0]), _lib.ptr(part), nf, _lib.stream())
+        (dq_, lddq), (dk_, lddk), (dv_, lddv) = grads
+        _lib.call("mx_packed_attn_bwd", q_, k_, v_, ldq, ldk, ldv, o_, ldo, do_, lddo, lse.data_ptr(),
+                  stats.data_ptr(), dq_, lddq, dk_, dv_, lddk, lddv, *seqs.ptrs, T, Hq, Hkv, D,
+                  D ** -0.5 if scale is None else scale, int(not given), _lib.ptr(part), nf, _lib.stream())
     return dq, dk, dv
 
 
