@@ -78,6 +78,18 @@ __device__ __forceinline__ uint32_t nonfinite(bf16x8 x) {   // high bit set in a
   return (((u.x & M) + A) | ((u.y & M) + A) | ((u.z & M) + A) | ((u.w & M) + A)) & 0x80008000u;
 }
 
+// Whether one of the lane's 16 rows (d: their -delta, 4 in 8) has a non-finite q or do.  delta = do . o
+// is not finite if do is not; nor if q is not, for then every score of the row, and so o, is not.
+__device__ __forceinline__ uint32_t bad_rows(const float* d) {
+  uint32_t bad = 0;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const float4 v = *reinterpret_cast<const float4*>(d + 8 * x);
+    bad |= !(fabsf(v.x) < INFINITY) | !(fabsf(v.y) < INFINITY) | !(fabsf(v.z) < INFINITY) | !(fabsf(v.w) < INFINITY);
+  }
+  return bad;
+}
+
 // Row-at-a-time forms for a wave whose masked subtiles met a non-finite operand: every lane holds
 // columns lane (+ 64) of the row, and only visible terms are ever formed.
 template <int D>
@@ -141,13 +153,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int tid = threadIdx.x, lane = tid & 63, wl = uni(tid >> 6);
   const int r = lane & 31, hh = lane >> 5, g = lane >> 4, gi = lane & 15;
   const int T = a.T, nqb = (T + BQ - 1) / BQ;
-  const int nv = uni(a.meta[0]);
   int rank, hq;
   block_map(a.Hq, rank, hq);
   const int hk = hq / (a.Hq / a.Hkv);
   const int q0 = (nqb - 1 - rank) * BQ;              // late blocks (most keys of a long sequence) first
   const int qw = q0 + 32 * wl, qrow = qw + r;
   uint16_t* outp = a.out + (size_t)qrow * a.ldout + hq * D;
+  // the table reads depend on nothing but the block (a row behind the last sequence has start = itself)
+  const int nv = uni(a.meta[0]);
+  const int qrow_c = min(qrow, T - 1);
+  const int kv_lo = uni(a.start[q0]) & ~31;
+  const int smin = uni(a.start[min(qw, T - 1)]), smax = uni(a.start[min(qw + 31, T - 1)]);
+  const int st = a.start[qrow_c];
   if (q0 >= nv) {                                    // behind the last sequence
     if (a.fill && qrow < T) {
       zero_row<D>(outp, hh);
@@ -156,15 +173,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     return;
   }
   const int q_end = min(q0 + BQ, nv);
-  const int kv_lo = uni(a.start[q0]) & ~31;
   const int ntile = (q_end - kv_lo + BK - 1) / BK;
   // the wave's rows: visible keys of row i are start(i) .. i
   const bool wave_on = qw < nv;
   const int wlast = min(qw + 31, nv - 1);
-  const int smin = uni(a.start[min(qw, nv - 1)]), smax = uni(a.start[wlast]);
-  const int qrow_c = min(qrow, nv - 1);
-  const int st = a.start[qrow_c];
   const int cnt = qrow < nv ? qrow - st + 1 : 0;     // visible keys
+
+  // DMA: per-lane byte offsets inside a tile
+  uint32_t voK[PPW], voV[PPW];
+#pragma unroll
+  for (int i = 0; i < PPW; ++i) {
+    const int R = (wl + 4 * i) * RPP + lane / CPR, ch = (lane % CPR) ^ swz<D>(R);
+    voK[i] = (uint32_t)(R * a.ldk + ch * 8) * 2u;
+    voV[i] = (uint32_t)(R * a.ldv + ch * 8) * 2u;
+  }
+  const uint16_t* kbase = a.k + (size_t)kv_lo * a.ldk + hk * D;
+  const uint16_t* vbase = a.v + (size_t)kv_lo * a.ldv + hk * D;
+  auto issue = [&](char* kd, char* vd, int j) __attribute__((always_inline)) {
+    const int rows = min(BK, nv - kv_lo - j * BK);
+    const i32x4_t kr = rows_rsrc<D>(kbase + (size_t)j * BK * a.ldk, rows, a.ldk);
+    const i32x4_t vr = rows_rsrc<D>(vbase + (size_t)j * BK * a.ldv, rows, a.ldv);
+#pragma unroll
+    for (int i = 0; i < PPW; ++i) {
+      dma16_buf(kr, voK[i], kd + (wl + 4 * i) * 1024);
+      dma16_buf(vr, voV[i], vd + (wl + 4 * i) * 1024);
+    }
+  };
+  issue(kbuf0, vbuf0, 0);                            // (under the row loads)
 
   bf16x8 qf[NKK];
   bf16x8 dof[DQ ? NKK : 1];
@@ -212,25 +247,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     offT[dt][0] = toff<D>(row0, col >> 3) + (col & 7) * 2;
     offT[dt][1] = toff<D>(row0 + 8, col >> 3) + (col & 7) * 2;
   }
-  uint32_t voK[PPW], voV[PPW];
-#pragma unroll
-  for (int i = 0; i < PPW; ++i) {
-    const int R = (wl + 4 * i) * RPP + lane / CPR, ch = (lane % CPR) ^ swz<D>(R);
-    voK[i] = (uint32_t)(R * a.ldk + ch * 8) * 2u;
-    voV[i] = (uint32_t)(R * a.ldv + ch * 8) * 2u;
-  }
-  const uint16_t* kbase = a.k + (size_t)kv_lo * a.ldk + hk * D;
-  const uint16_t* vbase = a.v + (size_t)kv_lo * a.ldv + hk * D;
-  auto issue = [&](char* kd, char* vd, int j) __attribute__((always_inline)) {
-    const int rows = min(BK, nv - kv_lo - j * BK);
-    const i32x4_t kr = rows_rsrc<D>(kbase + (size_t)j * BK * a.ldk, rows, a.ldk);
-    const i32x4_t vr = rows_rsrc<D>(vbase + (size_t)j * BK * a.ldv, rows, a.ldv);
-#pragma unroll
-    for (int i = 0; i < PPW; ++i) {
-      dma16_buf(kr, voK[i], kd + (wl + 4 * i) * 1024);
-      dma16_buf(vr, voV[i], vd + (wl + 4 * i) * 1024);
-    }
-  };
   const float c = a.c;
 
   auto seen = [&](int k0, int e) __attribute__((always_inline)) {   // key k0 + crow(e, hh) visible to the lane's row
@@ -355,7 +371,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if (j + 1 < ntile) issue(Kn, Vn, j + 1);
     compute(Kc, Vc, j);
   };
-  issue(kbuf0, vbuf0, 0);
   for (int j = 0; j < ntile; j += 2) {
     step(kbuf0, vbuf0, kbuf1, vbuf1, j);
     if (j + 1 < ntile) step(kbuf1, vbuf1, kbuf0, vbuf0, j + 1);
@@ -431,12 +446,17 @@ packed_kmajor_kernel(const PArgs a) {
   __shared__ __attribute__((aligned(16))) float db1[64];
   const int tid = threadIdx.x, lane = tid & 63, wl = uni(tid >> 6);
   const int r = lane & 31, hh = lane >> 5, g = lane >> 4, gi = lane & 15;
-  const int T = a.T, nv = uni(a.meta[0]);
+  const int T = a.T;
   int rank, hk;
   block_map(a.Hkv, rank, hk);
   const int grp = a.Hq / a.Hkv;
+  // (table reads that depend on the block alone; see packed_qmajor_kernel)
   const int k0 = rank * KB;                          // early blocks (most rows of a long sequence) first
   const int kw = k0 + 32 * wl, key = kw + r;
+  const int nv = uni(a.meta[0]);
+  const int qend = min(uni(a.end[min(k0 + KB, T) - 1]), nv);   // queries of the block: k0 .. qend - 1
+  const int emin = uni(a.end[min(kw, T - 1)]), emax = min(uni(a.end[min(kw + 31, T - 1)]), nv);
+  const int key_c = min(key, T - 1), kend = a.end[key_c];
   uint16_t* dkp = a.dk + (size_t)key * a.lddk + hk * D;
   uint16_t* dvp = a.dv + (size_t)key * a.lddv + hk * D;
   if (k0 >= nv) {
@@ -446,12 +466,39 @@ packed_kmajor_kernel(const PArgs a) {
     }
     return;
   }
-  const int qend = uni(a.end[min(k0 + KB, nv) - 1]);   // queries of the block: k0 .. qend - 1
   const int nqt = (qend - k0 + QT - 1) / QT, items = nqt * grp;
   const bool wave_on = kw < nv;
-  const int emin = uni(a.end[min(kw, nv - 1)]), emax = uni(a.end[min(kw + 31, nv - 1)]);
-  const int key_c = min(key, nv - 1);
-  const int cnt = key < nv ? a.end[key_c] - key : 0;   // rows that see this key: key .. key + cnt - 1
+  const int cnt = key < nv ? kend - key : 0;           // rows that see this key: key .. key + cnt - 1
+  uint32_t voQ[PPW], voO[PPW];
+#pragma unroll
+  for (int i = 0; i < PPW; ++i) {
+    const int R = (wl + 4 * i) * RPP + lane / CPR, ch = (lane % CPR) ^ swz<D>(R);
+    voQ[i] = (uint32_t)(R * a.ldq + ch * 8) * 2u;
+    voO[i] = (uint32_t)(R * a.lddo + ch * 8) * 2u;
+  }
+  auto issue = [&](char* qd, char* od, float* ld, float* dd, int hq, int qs) __attribute__((always_inline)) {
+    const int rows = min(QT, nv - qs);
+    const i32x4_t qr = rows_rsrc<D>(a.q + (size_t)qs * a.ldq + hq * D, rows, a.ldq);
+    const i32x4_t dr = rows_rsrc<D>(a.dout + (size_t)qs * a.lddo + hq * D, rows, a.lddo);
+#pragma unroll
+    for (int i = 0; i < PPW; ++i) {
+      dma16_buf(qr, voQ[i], qd + (wl + 4 * i) * 1024);
+      dma16_buf(dr, voO[i], od + (wl + 4 * i) * 1024);
+    }
+    if (wl < 2) {
+      const size_t li = (size_t)hq * T + min(qs + lane, nv - 1);
+      if (wl == 0) dma4(a.nlse + li, (char*)ld);
+      else dma4(a.delta + li, (char*)dd);
+    }
+  };
+  int hq_n = hk * grp, qs_n = k0;      // the item to fetch next
+  int qs_c = k0;
+  auto advance = [&]() __attribute__((always_inline)) {
+    qs_n += QT;
+    if (qs_n >= qend) { qs_n = k0; ++hq_n; }
+  };
+  issue(qb0, ob0, lb0, db0, hq_n, qs_n);             // (under the row loads)
+  advance();
   bf16x8 kf[NKK], vf[NKK];
   {
     const uint16_t* kp = a.k + (size_t)key_c * a.ldk + hk * D + 8 * hh;
@@ -477,28 +524,6 @@ packed_kmajor_kernel(const PArgs a) {
     offT[dt][0] = toff<D>(row0, col >> 3) + (col & 7) * 2;
     offT[dt][1] = toff<D>(row0 + 8, col >> 3) + (col & 7) * 2;
   }
-  uint32_t voQ[PPW], voO[PPW];
-#pragma unroll
-  for (int i = 0; i < PPW; ++i) {
-    const int R = (wl + 4 * i) * RPP + lane / CPR, ch = (lane % CPR) ^ swz<D>(R);
-    voQ[i] = (uint32_t)(R * a.ldq + ch * 8) * 2u;
-    voO[i] = (uint32_t)(R * a.lddo + ch * 8) * 2u;
-  }
-  auto issue = [&](char* qd, char* od, float* ld, float* dd, int hq, int qs) __attribute__((always_inline)) {
-    const int rows = min(QT, nv - qs);
-    const i32x4_t qr = rows_rsrc<D>(a.q + (size_t)qs * a.ldq + hq * D, rows, a.ldq);
-    const i32x4_t dr = rows_rsrc<D>(a.dout + (size_t)qs * a.lddo + hq * D, rows, a.lddo);
-#pragma unroll
-    for (int i = 0; i < PPW; ++i) {
-      dma16_buf(qr, voQ[i], qd + (wl + 4 * i) * 1024);
-      dma16_buf(dr, voO[i], od + (wl + 4 * i) * 1024);
-    }
-    if (wl < 2) {
-      const size_t li = (size_t)hq * T + min(qs + lane, nv - 1);
-      if (wl == 0) dma4(a.nlse + li, (char*)ld);
-      else dma4(a.delta + li, (char*)dd);
-    }
-  };
   const float c = a.c;
   uint32_t bad = 0;   // (see packed_qmajor_kernel)
   auto body = [&](const char* Qt, const char* Ot, const float* Lt, const float* Dt, int qs) __attribute__((always_inline)) {
@@ -536,8 +561,7 @@ packed_kmajor_kernel(const PArgs a) {
           s[e] = seen ? s[e] : 0.f;
           dp[e] = seen ? dp[e] : 0.f;
         }
-#pragma unroll
-        for (int kk = 0; kk < NKK; ++kk) bad |= nonfinite(lds8(Qu, offQ[kk])) | nonfinite(lds8(Ou, offQ[kk]));
+        bad |= bad_rows(Dt + 32 * u + 4 * hh);
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -552,12 +576,6 @@ packed_kmajor_kernel(const PArgs a) {
       }
     }
   };
-  int hq_n = hk * grp, qs_n = k0;      // the item to fetch next
-  int qs_c = k0;
-  auto advance = [&]() __attribute__((always_inline)) {
-    qs_n += QT;
-    if (qs_n >= qend) { qs_n = k0; ++hq_n; }
-  };
   auto step = [&](char* Qc, char* Oc, float* Lc, float* Dc, char* Qn, char* On, float* Ln, float* Dn,
                   int t) __attribute__((always_inline)) {
     vm_drain();
@@ -570,8 +588,6 @@ packed_kmajor_kernel(const PArgs a) {
     }
     if (uni(wave_on && qs < emax && qs + QT > kw ? 1 : 0)) body(Qc, Oc, Lc, Dc, qs);
   };
-  issue(qb0, ob0, lb0, db0, hq_n, qs_n);
-  advance();
   for (int t = 0; t < items; t += 2) {
     step(qb0, ob0, lb0, db0, qb1, ob1, lb1, db1, t);
     if (t + 1 < items) step(qb1, ob1, lb1, db1, qb0, ob0, lb0, db0, t + 1);
@@ -642,12 +658,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   __shared__ __attribute__((aligned(16))) uint4 vlds[4][2 * NL][64];  // the waves' V fragments of odd kk
   const int tid = threadIdx.x, lane = tid & 63, wl = uni(tid >> 6);
   const int r = lane & 31, hh = lane >> 5, g = lane >> 4, gi = lane & 15;
-  const int T = a.T, nv = uni(a.meta[0]);
+  const int T = a.T;
   const int nblk = gridDim.x / a.nsplit, sp = blockIdx.x / nblk;
   int rank, hk;
   block_map(blockIdx.x - sp * nblk, a.Hkv, rank, hk);
   const int grp = a.Hq / a.Hkv;
   const int k0 = rank * KB2, kw = k0 + 64 * wl;
+  const int nv = uni(a.meta[0]);
+  const int qend = min(uni(a.end[min(k0 + KB2, T) - 1]), nv);
+  const int emax = min(uni(a.end[min(kw + 63, T - 1)]), nv);
+  int key[2], cnt[2], emin[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    key[j] = kw + 32 * j + r;
+    cnt[j] = a.end[min(key[j], T - 1)] - key[j];       // rows that see this key: key .. key + cnt - 1
+    emin[j] = uni(a.end[min(kw + 32 * j, T - 1)]);
+  }
   if (k0 >= nv) {
     if (a.fill && sp == 0)
       for (int key = kw + r; key < min(kw + 64, T); key += 32) {
@@ -656,23 +682,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       }
     return;
   }
-  const int qend = uni(a.end[min(k0 + KB2, nv) - 1]);
   const int nqt = (qend - k0 + QT - 1) / QT, items = nqt * grp;
   const int nsp = block_splits(items, a.nsplit), per = (items + nsp - 1) / nsp;
   const int t0 = sp * per, t1 = min(items, t0 + per);
   if (sp >= nsp) return;
   const bool wave_on = kw < nv;
   const int klast = min(kw + 63, nv - 1);
-  const int emax = uni(a.end[max(klast, 0)]);
-  int key[2], cnt[2], emin[2];
   uint32_t bad = 0;   // (see packed_qmajor_kernel)
   bf16x8 kf[2][NKK], vf[2][NL];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    key[j] = kw + 32 * j + r;
+    if (key[j] >= nv) cnt[j] = 0;
     const int kc = min(key[j], nv - 1);
-    cnt[j] = key[j] < nv ? a.end[kc] - key[j] : 0;     // rows that see this key: key .. key + cnt - 1
-    emin[j] = uni(a.end[min(kw + 32 * j, nv - 1)]);
     const uint16_t* kp = a.k + (size_t)kc * a.ldk + hk * D + 8 * hh;
     const uint16_t* vp = a.v + (size_t)kc * a.ldv + hk * D + 8 * hh;
 #pragma unroll
@@ -802,20 +823,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       };
       if (part) {
         // P = 0 where masked; dS = P (dP - delta) is then 0 too unless a factor is not finite, which marks
-        // the wave (dO, Q and delta here; its V rows were looked at when they were loaded)
+        // the wave (bad_rows here; its V rows were looked at when they were loaded)
         asm volatile("" ::: "memory");   // a real branch
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             s[j][e] = (uint32_t)(qsu + 4 * hh - key[j] + crow(e, 0)) < (uint32_t)cnt[j] ? s[j][e] : 0.f;
-#pragma unroll
-        for (int kk = 0; kk < NKK; ++kk) bad |= nonfinite(rread(Qu, kk)) | nonfinite(rread(Ou, kk));
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const float2 de = *reinterpret_cast<const float2*>(Du + 8 * (x >> 1) + 2 * (x & 1));
-          bad |= !(fabsf(de.x) < INFINITY) || !(fabsf(de.y) < INFINITY) ? 0x8000u : 0u;
-        }
+        bad |= bad_rows(Du);
       }
       bf16x8 w[2][2];                                  // P, then dS, of both groups as MFMA operands
 #pragma unroll
@@ -946,7 +961,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PArgs a) {
   const int nv = a.meta[0];
   if (t >= nv) return;
   const int col = (int)(v - t * nw) * 4, k0 = (int)t / KB2 * KB2;
-  const int nqt = (a.end[min(k0 + KB2, nv) - 1] - k0 + QT2 - 1) / QT2;
+  const int nqt = (min(a.end[min(k0 + KB2, a.T) - 1], nv) - k0 + QT2 - 1) / QT2;
   const int nsp = block_splits(nqt * (a.Hq / a.Hkv), a.nsplit);
   if (nsp == 1) return;
 #pragma unroll
