@@ -59,15 +59,51 @@ __global__ __launch_bounds__(256) void packed_plan_kernel(const IT* __restrict__
   pos[t] = t - s;
 }
 
+// Dispatch order of the 128-row query blocks, the 128-key and the 256-key blocks: most work first
+// (ties: query blocks from the back, key blocks from the front), so that the longest blocks of a batch
+// of mixed lengths do not start last.  One workgroup counts each block's rank; order: [nq][nk][nk2].
+// Above ORDER_MAX blocks the lists are left in sequence order.
+constexpr int ORDER_MAX = 2048;
+__global__ __launch_bounds__(1024) void packed_order_kernel(int T, const int* __restrict__ start,
+                                                            const int* __restrict__ end, const int* __restrict__ meta,
+                                                            int* __restrict__ order) {
+  __shared__ int work[ORDER_MAX];
+  const int nv = meta[0], tid = threadIdx.x;
+#pragma unroll 1
+  for (int list = 0; list < 3; ++list) {
+    const int B = list == 2 ? 256 : 128, nb = (T + B - 1) / B;
+    if (nb > ORDER_MAX) {
+      for (int b = tid; b < nb; b += 1024) order[b] = list == 0 ? nb - 1 - b : b;
+    } else {
+      for (int b = tid; b < nb; b += 1024) {
+        const int b0 = b * B, b1 = min(b0 + B, nv);
+        work[b] = b0 >= nv ? 0 : list == 0 ? b1 - start[b0] : end[b1 - 1] - b0;
+      }
+      __syncthreads();
+      for (int b = tid; b < nb; b += 1024) {
+        const int w = work[b];
+        int rank = 0;
+#pragma unroll 16
+        for (int o = 0; o < nb; ++o)
+          rank += (int)(work[o] > w) | ((int)(work[o] == w) & (int)(list == 0 ? o > b : o < b));
+        order[rank] = b;
+      }
+      __syncthreads();
+    }
+    order += nb;
+  }
+}
+
 struct PArgs {
   const uint16_t *q, *k, *v, *dout, *o;
   uint16_t *out, *dk, *dv;      // forward: O; backward: dQ, dK, dV
   float *lse, *nlse, *delta;    // [Hq][T]: log-sum-exp; backward: -lse / c and -delta
   const int *start, *end, *meta;
+  const int* order;             // the launched kernel's dispatch order
   int ldq, ldk, ldv, lddo, ldo, ldout, lddk, lddv;
   int T, Hq, Hkv;
   float c, scale;               // scale log2(e), scale
-  float* part;                  // D = 128: partial dK / dV of split blocks
+  float* part;                  // partial dK / dV of split blocks
   int nsplit;
   int fill;                     // zero the rows behind the last sequence (else leave them)
 };
@@ -138,6 +174,13 @@ __device__ __forceinline__ void zero_row(uint16_t* row, int hh) {   // the lane'
   for (int i = 0; i < D / 16; ++i) *reinterpret_cast<uint4*>(row + 16 * i + 8 * hh) = make_uint4(0, 0, 0, 0);
 }
 
+// When every workgroup is resident at once (two on each of the 256 CUs), the CU that got the heaviest
+// gets its second from the light end; else the hardware's dispatch in descending order balances.
+__device__ __forceinline__ int pair_rank(int rank, int n) {
+  const int half = (n + 1) / 2;
+  return gridDim.x <= 512 && rank >= half ? n - 1 - (rank - half) : rank;
+}
+
 // ============================================================================ query-major
 // Forward, and dQ of the backward.  Four waves of 32 query rows; query on the MFMA lane
 // (S^T = K Q^T, O^T = V^T P^T), so the softmax statistics are lane-local plus one half exchange.
@@ -156,7 +199,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   int rank, hq;
   block_map(a.Hq, rank, hq);
   const int hk = hq / (a.Hq / a.Hkv);
-  const int q0 = (nqb - 1 - rank) * BQ;              // late blocks (most keys of a long sequence) first
+  const int q0 = uni(a.order[pair_rank(rank, nqb)]) * BQ;
   const int qw = q0 + 32 * wl, qrow = qw + r;
   uint16_t* outp = a.out + (size_t)qrow * a.ldout + hq * D;
   // the table reads depend on nothing but the block (a row behind the last sequence has start = itself)
@@ -441,12 +484,92 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 }
 
 // ============================================================================ key-major
-// dK, dV, D = 64.  Four waves of 32 keys, key on the MFMA lane; Q / dO tiles of QT rows (and their lse,
-// delta) stream through a two-slot LDS-DMA ring, over the query heads of the key head's group.
+constexpr int KB1 = 128, KB2 = 256, QT2 = 64;   // keys of a block (D = 64 / 128), rows of a query tile
+constexpr int SPLIT_MIN = 24;                   // fewest items of a split
+__device__ __forceinline__ int block_splits(int items, int nsplit) { return max(1, min(nsplit, items / SPLIT_MIN)); }
+
+// Where a key block's dK / dV go: the results, or fp32 partials of its split [split][dk, dv][T][Hkv D]
+template <int D>
+struct KeyOut {
+  const PArgs& a;
+  int hk, nsp, lane, W;
+  float *pk, *pv;
+  __device__ __forceinline__ KeyOut(const PArgs& a_, int hk_, int sp, int nsp_, int lane_)
+      : a(a_), hk(hk_), nsp(nsp_), lane(lane_), W(a_.Hkv * D) {
+    pk = a.part + (size_t)sp * 2 * a.T * W + hk * D;
+    pv = pk + (size_t)a.T * W;
+  }
+  // the accumulators of one key per lane pair
+  template <int N>
+  __device__ __forceinline__ void put(int key, const f32x16 (&dk)[N], const f32x16 (&dv)[N], int hh) const {
+    if (nsp > 1) {
+#pragma unroll
+      for (int dt = 0; dt < N; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const size_t o = (size_t)key * W + 32 * dt + 2 * e + 4 * hh;
+          *reinterpret_cast<float4*>(pk + o) = make_float4(dk[dt][e], dk[dt][e + 1], dk[dt][e + 2], dk[dt][e + 3]);
+          *reinterpret_cast<float4*>(pv + o) = make_float4(dv[dt][e], dv[dt][e + 1], dv[dt][e + 2], dv[dt][e + 3]);
+        }
+      return;
+    }
+#pragma unroll
+    for (int dt = 0; dt < N; ++dt) {
+      store_row32(a.dk + (size_t)key * a.lddk + hk * D + 32 * dt, dk[dt], a.scale, hh);
+      store_row32(a.dv + (size_t)key * a.lddv + hk * D + 32 * dt, dv[dt], 1.f, hh);
+    }
+  }
+  __device__ __forceinline__ void put(int key, const RowVec<D>& dk, const RowVec<D>& dv) const {
+    if (nsp > 1) {
+#pragma unroll
+      for (int x = 0; x < D / 64; ++x) {
+        pk[(size_t)key * W + lane + 64 * x] = dk.x[x];
+        pv[(size_t)key * W + lane + 64 * x] = dv.x[x];
+      }
+      return;
+    }
+    dk.store(a.dk + (size_t)key * a.lddk + hk * D, lane, a.scale);
+    dv.store(a.dv + (size_t)key * a.lddv + hk * D, lane, 1.f);
+  }
+};
+
+// keys ka .. kb one by one over the items t0 .. t1 - 1 of their block (a wave that met a non-finite operand)
+template <int D>
+__device__ __forceinline__ void redo_keys(const PArgs& a, const KeyOut<D>& out, int ka, int kb, int k0, int t0, int t1,
+                                          int nqt, int hk, int grp, int lane) {
+#pragma unroll 1
+  for (int j = ka; j <= kb; ++j) {
+    const RowVec<D> kj(a.k + (size_t)j * a.ldk + hk * D, lane);
+    const RowVec<D> vj(a.v + (size_t)j * a.ldv + hk * D, lane);
+    RowVec<D> rk, rv;
+    const int je = a.end[j];
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {
+      const int hq = hk * grp + t / nqt, qs = k0 + (t % nqt) * QT2;
+#pragma unroll 1
+      for (int i = max(j, qs); i < min(je, qs + QT2); ++i) {
+        const RowVec<D> qi(a.q + (size_t)i * a.ldq + hq * D, lane);
+        const RowVec<D> doi(a.dout + (size_t)i * a.lddo + hq * D, lane);
+        const size_t li = (size_t)hq * a.T + i;
+        const float pij = __builtin_amdgcn_exp2f(__builtin_fmaf(qi.dot(kj), a.c, -a.lse[li]));
+        rv.axpy(pij, doi);
+        rk.axpy(pij * (doi.dot(vj) + a.delta[li]), qi);
+      }
+    }
+    out.put(j, rk, rv);
+  }
+}
+
+// dK, dV: key on the MFMA lane; Q / dO tiles of QT rows (and their statistics) stream through a
+// two-slot LDS-DMA ring, over the query heads of the key head's group.  Where there are few key blocks,
+// those of long sequences are split along their (query head, query tile) items over up to `nsplit`
+// workgroups, whose fp32 partial sums packed_join_kernel adds in order.
+//
+// D = 64.  Four waves of 32 keys, two waves per SIMD.
 template <int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void
 packed_kmajor_kernel(const PArgs a) {
-  constexpr int KB = 128, QT = 64, NQS = QT / 32, NKK = D / 16, NDT = D / 32;
+  constexpr int KB = KB1, QT = QT2, NQS = QT / 32, NKK = D / 16, NDT = D / 32;
   constexpr int RB = D * 2, CPR = D / 8, RPP = 64 / CPR, TILE = QT * RB, PPW = TILE / 1024 / 4;
   __shared__ __attribute__((aligned(16))) char qb0[TILE];
   __shared__ __attribute__((aligned(16))) char qb1[TILE];
@@ -459,11 +582,12 @@ packed_kmajor_kernel(const PArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wl = uni(tid >> 6);
   const int r = lane & 31, hh = lane >> 5, g = lane >> 4, gi = lane & 15;
   const int T = a.T;
+  const int nblk = gridDim.x / a.nsplit, sp = blockIdx.x / nblk;
   int rank, hk;
-  block_map(a.Hkv, rank, hk);
+  block_map(blockIdx.x - sp * nblk, a.Hkv, rank, hk);
   const int grp = a.Hq / a.Hkv;
   // (table reads that depend on the block alone; see packed_qmajor_kernel)
-  const int k0 = rank * KB;                          // early blocks (most rows of a long sequence) first
+  const int k0 = uni(a.order[pair_rank(rank, (T + KB - 1) / KB)]) * KB;
   const int kw = k0 + 32 * wl, key = kw + r;
   const int nv = uni(a.meta[0]);
   const int qend = min(uni(a.end[min(k0 + KB, T) - 1]), nv);   // queries of the block: k0 .. qend - 1
@@ -472,13 +596,16 @@ packed_kmajor_kernel(const PArgs a) {
   uint16_t* dkp = a.dk + (size_t)key * a.lddk + hk * D;
   uint16_t* dvp = a.dv + (size_t)key * a.lddv + hk * D;
   if (k0 >= nv) {
-    if (a.fill && key < T) {
+    if (a.fill && sp == 0 && key < T) {
       zero_row<D>(dkp, hh);
       zero_row<D>(dvp, hh);
     }
     return;
   }
   const int nqt = (qend - k0 + QT - 1) / QT, items = nqt * grp;
+  const int nsp = block_splits(items, a.nsplit), per = (items + nsp - 1) / nsp;
+  const int t0 = sp * per, t1 = min(items, t0 + per);
+  if (sp >= nsp) return;
   const bool wave_on = kw < nv;
   const int cnt = key < nv ? kend - key : 0;           // rows that see this key: key .. key + cnt - 1
   uint32_t voQ[PPW], voO[PPW];
@@ -503,8 +630,8 @@ packed_kmajor_kernel(const PArgs a) {
       else dma4(a.delta + li, (char*)dd);
     }
   };
-  int hq_n = hk * grp, qs_n = k0;      // the item to fetch next
-  int qs_c = k0;
+  int hq_n = hk * grp + t0 / nqt, qs_n = k0 + (t0 % nqt) * QT;   // the item to fetch next
+  int qs_c = qs_n;
   auto advance = [&]() __attribute__((always_inline)) {
     qs_n += QT;
     if (qs_n >= qend) { qs_n = k0; ++hq_n; }
@@ -593,61 +720,35 @@ packed_kmajor_kernel(const PArgs a) {
     vm_drain();
     __syncthreads();
     const int qs = qs_c;
-    if (t + 1 < items) {
+    if (t + 1 < t1) {
       issue(Qn, On, Ln, Dn, hq_n, qs_n);
       qs_c = qs_n;
       advance();
     }
     if (uni(wave_on && qs < emax && qs + QT > kw ? 1 : 0)) body(Qc, Oc, Lc, Dc, qs);
   };
-  for (int t = 0; t < items; t += 2) {
+  for (int t = t0; t < t1; t += 2) {
     step(qb0, ob0, lb0, db0, qb1, ob1, lb1, db1, t);
-    if (t + 1 < items) step(qb1, ob1, lb1, db1, qb0, ob0, lb0, db0, t + 1);
+    if (t + 1 < t1) step(qb1, ob1, lb1, db1, qb0, ob0, lb0, db0, t + 1);
   }
-  if (a.fill && key >= nv && key < T) {
+  if (a.fill && sp == 0 && key >= nv && key < T) {
     zero_row<D>(dkp, hh);
     zero_row<D>(dvp, hh);
   }
+  const KeyOut<D> out(a, hk, sp, nsp, lane);
   if (__any(bad != 0)) {
-#pragma unroll 1
-    for (int j = kw; j <= min(kw + 31, nv - 1); ++j) {
-      const RowVec<D> kj(a.k + (size_t)j * a.ldk + hk * D, lane);
-      const RowVec<D> vj(a.v + (size_t)j * a.ldv + hk * D, lane);
-      RowVec<D> rk, rv;
-      const int je = a.end[j];
-#pragma unroll 1
-      for (int hq = hk * grp; hq < hk * grp + grp; ++hq)
-#pragma unroll 1
-        for (int i = j; i < je; ++i) {
-          const RowVec<D> qi(a.q + (size_t)i * a.ldq + hq * D, lane);
-          const RowVec<D> doi(a.dout + (size_t)i * a.lddo + hq * D, lane);
-          const size_t li = (size_t)hq * T + i;
-          const float pij = __builtin_amdgcn_exp2f(__builtin_fmaf(qi.dot(kj), c, -a.lse[li]));
-          rv.axpy(pij, doi);
-          rk.axpy(pij * (doi.dot(vj) + a.delta[li]), qi);
-        }
-      rk.store(a.dk + (size_t)j * a.lddk + hk * D, lane, a.scale);
-      rv.store(a.dv + (size_t)j * a.lddv + hk * D, lane, 1.f);
-    }
+    redo_keys<D>(a, out, kw, min(kw + 31, nv - 1), k0, t0, t1, nqt, hk, grp, lane);
     return;
   }
   if (key >= nv) return;
-#pragma unroll
-  for (int dt = 0; dt < NDT; ++dt) {
-    store_row32(dkp + 32 * dt, dkacc[dt], a.scale, hh);
-    store_row32(dvp + 32 * dt, dvacc[dt], 1.f, hh);
-  }
+  out.put(key, dkacc, dvacc, hh);
 }
 
 // D = 128.  Two 32-key groups per wave, one wave per SIMD: every Q / dO fragment read from LDS feeds
 // two MFMAs (a 32-key wave needs 1408 LDS cycles per 1024 MFMA cycles of the four SIMDs -- the
 // transposed reads run at half rate --, this one 1408 per 2048), and the accumulators of both groups
 // (256 registers), their K and V rows (128) and S, dP (64) just fit the 512 registers.
-// A workgroup holds 256 keys.  Blocks of long sequences are split along their (query head, query
-// tile) items over up to `nsplit` workgroups, whose fp32 partial sums packed_join_kernel adds in order.
-constexpr int KB2 = 256, QT2 = 64, SPLIT_MIN = 24;   // fewest items of a split
-__device__ __forceinline__ int block_splits(int items, int nsplit) { return max(1, min(nsplit, items / SPLIT_MIN)); }
-
+// A workgroup holds 256 keys.
 // MFMA with its accumulator in ordinary registers.  The compiler gives every MFMA of a kernel that
 // needs accumulation registers an accumulator there; dK and dV of 64 keys take all 256 of them, and
 // it moved S and dP in and out of them at every subtile.  Written as asm, so the wait between the
@@ -675,7 +776,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   int rank, hk;
   block_map(blockIdx.x - sp * nblk, a.Hkv, rank, hk);
   const int grp = a.Hq / a.Hkv;
-  const int k0 = rank * KB2, kw = k0 + 64 * wl;
+  const int k0 = uni(a.order[rank]) * KB2, kw = k0 + 64 * wl;
   const int nv = uni(a.meta[0]);
   const int qend = min(uni(a.end[min(k0 + KB2, T) - 1]), nv);
   const int emax = min(uni(a.end[min(kw + 63, T - 1)]), nv);
@@ -896,70 +997,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     if (uni(wave_on && qs < emax && qs + QT > kw ? 1 : 0))
       body(ring[slot], ring[slot] + TILE, stat[slot][0], stat[slot][1], qs);
   }
-  const int W = a.Hkv * D;
-  float* pk = a.part + (size_t)sp * 2 * T * W + hk * D;   // [split][dk, dv][T][Hkv D]
-  float* pv = pk + (size_t)T * W;
-  if (__any(bad != 0)) {
-#pragma unroll 1
-    for (int j = kw; j <= klast; ++j) {
-      const RowVec<D> kj(a.k + (size_t)j * a.ldk + hk * D, lane);
-      const RowVec<D> vj(a.v + (size_t)j * a.ldv + hk * D, lane);
-      RowVec<D> rk, rv;
-      const int je = a.end[j];
-#pragma unroll 1
-      for (int t = t0; t < t1; ++t) {
-        const int hq = hk * grp + t / nqt, qs = k0 + (t % nqt) * QT;
-#pragma unroll 1
-        for (int i = max(j, qs); i < min(je, qs + QT); ++i) {
-          const RowVec<D> qi(a.q + (size_t)i * a.ldq + hq * D, lane);
-          const RowVec<D> doi(a.dout + (size_t)i * a.lddo + hq * D, lane);
-          const size_t li = (size_t)hq * T + i;
-          const float pij = __builtin_amdgcn_exp2f(__builtin_fmaf(qi.dot(kj), c, -a.lse[li]));
-          rv.axpy(pij, doi);
-          rk.axpy(pij * (doi.dot(vj) + a.delta[li]), qi);
-        }
-      }
-      if (nsp > 1) {
-#pragma unroll
-        for (int x = 0; x < D / 64; ++x) {
-          pk[(size_t)j * W + lane + 64 * x] = rk.x[x];
-          pv[(size_t)j * W + lane + 64 * x] = rv.x[x];
-        }
-      } else {
-        rk.store(a.dk + (size_t)j * a.lddk + hk * D, lane, a.scale);
-        rv.store(a.dv + (size_t)j * a.lddv + hk * D, lane, 1.f);
-      }
-    }
-  }
+  const KeyOut<D> out(a, hk, sp, nsp, lane);
+  const bool redo = __any(bad != 0);
+  if (redo) redo_keys<D>(a, out, kw, klast, k0, t0, t1, nqt, hk, grp, lane);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    uint16_t* dkp = a.dk + (size_t)key[j] * a.lddk + hk * D;
-    uint16_t* dvp = a.dv + (size_t)key[j] * a.lddv + hk * D;
     if (key[j] >= nv) {
       if (a.fill && sp == 0 && key[j] < T) {
-        zero_row<D>(dkp, hh);
-        zero_row<D>(dvp, hh);
+        zero_row<D>(a.dk + (size_t)key[j] * a.lddk + hk * D, hh);
+        zero_row<D>(a.dv + (size_t)key[j] * a.lddv + hk * D, hh);
       }
-      continue;
-    }
-    if (__any(bad != 0)) continue;
-    if (nsp > 1) {
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const size_t o = (size_t)key[j] * W + 32 * dt + 2 * e + 4 * hh;
-          *reinterpret_cast<float4*>(pk + o) =
-              make_float4(dkacc[j][dt][e], dkacc[j][dt][e + 1], dkacc[j][dt][e + 2], dkacc[j][dt][e + 3]);
-          *reinterpret_cast<float4*>(pv + o) =
-              make_float4(dvacc[j][dt][e], dvacc[j][dt][e + 1], dvacc[j][dt][e + 2], dvacc[j][dt][e + 3]);
-        }
-    } else {
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) {
-        store_row32(dkp + 32 * dt, dkacc[j][dt], a.scale, hh);
-        store_row32(dvp + 32 * dt, dvacc[j][dt], 1.f, hh);
-      }
+    } else if (!redo) {
+      out.put(key[j], dkacc[j], dvacc[j], hh);
     }
   }
 }
@@ -972,8 +1021,9 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PArgs a) {
   const int64_t t = v / nw;
   const int nv = a.meta[0];
   if (t >= nv) return;
-  const int col = (int)(v - t * nw) * 4, k0 = (int)t / KB2 * KB2;
-  const int nqt = (min(a.end[min(k0 + KB2, a.T) - 1], nv) - k0 + QT2 - 1) / QT2;
+  constexpr int KB = D == 64 ? KB1 : KB2;
+  const int col = (int)(v - t * nw) * 4, k0 = (int)t / KB * KB;
+  const int nqt = (min(a.end[min(k0 + KB, a.T) - 1], nv) - k0 + QT2 - 1) / QT2;
   const int nsp = block_splits(nqt * (a.Hq / a.Hkv), a.nsplit);
   if (nsp == 1) return;
 #pragma unroll
@@ -989,11 +1039,12 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PArgs a) {
   }
 }
 
-// splits of the D = 128 key blocks: enough workgroups for four rounds of the 256 CUs
-int key_splits(int T, int Hkv) {
-  const int64_t blocks = (int64_t)((T + KB2 - 1) / KB2) * Hkv;
+// splits of the key blocks: enough workgroups for several rounds of the chip
+int key_splits(int T, int Hkv, int D) {
+  const int kb = D == 64 ? KB1 : KB2;
+  const int64_t blocks = (int64_t)((T + kb - 1) / kb) * Hkv;
   int n = 1;
-  while (n < 4 && blocks * n < 1024) n *= 2;
+  while (n < (D == 64 ? 8 : 4) && blocks * n < (D == 64 ? 512 : 1024)) n *= 2;
   return n;
 }
 
@@ -1010,8 +1061,8 @@ bool bad_shape(int T, int Hq, int Hkv, int D) {
 // Row table of a packed batch (packed_plan_kernel).  cu: n + 1 cumulative lengths (int64 when
 // `wide`, else int32); start, end: int32 [T]; meta: int32 [4]; pos: int64 [T].
 MX_EXPORT int mx_packed_plan(const void* cu, int wide, int n, int T, int* start, int* end, int* meta, void* pos,
-                             hipStream_t s) {
-  if (!cu || !start || !end || !meta || !pos || n < 1 || T <= 0 || T > (1 << 30)) return hipErrorInvalidValue;
+                             int* order, hipStream_t s) {
+  if (!cu || !start || !end || !meta || !pos || !order || n < 1 || T <= 0 || T > (1 << 30)) return hipErrorInvalidValue;
   const dim3 grid((T + 255) / 256);
   if (wide)
     hipLaunchKernelGGL((packed_plan_kernel<int64_t>), grid, dim3(256), 0, s, (const int64_t*)cu, n, T, start, end,
@@ -1019,22 +1070,26 @@ MX_EXPORT int mx_packed_plan(const void* cu, int wide, int n, int T, int* start,
   else
     hipLaunchKernelGGL((packed_plan_kernel<int32_t>), grid, dim3(256), 0, s, (const int32_t*)cu, n, T, start, end,
                        meta, (int64_t*)pos);
+  hipLaunchKernelGGL(packed_order_kernel, dim3(1), dim3(1024), 0, s, T, start, end, meta, order);
   return hipGetLastError();
 }
+
+// int32 entries of `order` for T rows
+MX_EXPORT int64_t mx_packed_order_len(int T) { return T > 0 ? 2 * ((int64_t)(T + 127) / 128) + (T + 255) / 256 : 0; }
 
 // Q, K, V, O: bf16 [T] rows with strides ld*, head h at column h D.  lse: fp32 [Hq][T], base 2.
 // fill: rows behind the last sequence get o = 0, lse = +inf; else they are left as they are.
 MX_EXPORT int mx_packed_attn_fwd(const void* q, const void* k, const void* v, int ldq, int ldk, int ldv, void* o,
-                                 int ldo, float* lse, const int* start, const int* end, const int* meta, int T,
-                                 int Hq, int Hkv, int D, float scale, int fill, hipStream_t s) {
+                                 int ldo, float* lse, const int* start, const int* end, const int* meta, const int* order,
+                                 int T, int Hq, int Hkv, int D, float scale, int fill, hipStream_t s) {
   if (bad_shape(T, Hq, Hkv, D) || bad_mat(q, ldq, Hq * D) || bad_mat(k, ldk, Hkv * D) || bad_mat(v, ldv, Hkv * D) ||
-      bad_mat(o, ldo, Hq * D) || !lse || !start || !end || !meta || !(scale > 0.f))
+      bad_mat(o, ldo, Hq * D) || !lse || !start || !end || !meta || !order || !(scale > 0.f))
     return hipErrorInvalidValue;
   PArgs a{};
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
   a.out = (uint16_t*)o;
   a.lse = lse;
-  a.start = start; a.end = end; a.meta = meta;
+  a.start = start; a.end = end; a.meta = meta; a.order = order;
   a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldout = ldo;
   a.T = T; a.Hq = Hq; a.Hkv = Hkv;
   a.c = scale * 1.4426950408889634f;
@@ -1048,8 +1103,8 @@ MX_EXPORT int mx_packed_attn_fwd(const void* q, const void* k, const void* v, in
 
 // floats of `part` (0: none)
 MX_EXPORT int64_t mx_packed_attn_bwd_floats(int T, int Hkv, int D) {
-  if (T <= 0 || Hkv <= 0 || D != 128) return 0;
-  const int n = key_splits(T, Hkv);
+  if (T <= 0 || Hkv <= 0 || (D != 64 && D != 128)) return 0;
+  const int n = key_splits(T, Hkv, D);
   return n > 1 ? (int64_t)n * 2 * T * Hkv * D : 0;
 }
 
@@ -1057,12 +1112,12 @@ MX_EXPORT int64_t mx_packed_attn_bwd_floats(int T, int Hkv, int D) {
 MX_EXPORT int mx_packed_attn_bwd(const void* q, const void* k, const void* v, int ldq, int ldk, int ldv,
                                  const void* o, int ldo, const void* dout, int lddo, const float* lse, float* stats,
                                  void* dq, int lddq, void* dk, void* dv, int lddk, int lddv, const int* start,
-                                 const int* end, const int* meta, int T, int Hq, int Hkv, int D, float scale,
-                                 int fill, float* part, int64_t part_floats, hipStream_t s) {
+                                 const int* end, const int* meta, const int* order, int T, int Hq, int Hkv, int D,
+                                 float scale, int fill, float* part, int64_t part_floats, hipStream_t s) {
   if (bad_shape(T, Hq, Hkv, D) || bad_mat(q, ldq, Hq * D) || bad_mat(k, ldk, Hkv * D) || bad_mat(v, ldv, Hkv * D) ||
       bad_mat(o, ldo, Hq * D) || bad_mat(dout, lddo, Hq * D) || bad_mat(dq, lddq, Hq * D) ||
       bad_mat(dk, lddk, Hkv * D) || bad_mat(dv, lddv, Hkv * D) || !lse || !stats || ((uintptr_t)stats & 3) || !start ||
-      !end || !meta || !(scale > 0.f))
+      !end || !meta || !order || !(scale > 0.f))
     return hipErrorInvalidValue;
   PArgs a{};
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
@@ -1071,28 +1126,31 @@ MX_EXPORT int mx_packed_attn_bwd(const void* q, const void* k, const void* v, in
   a.lse = const_cast<float*>(lse);
   a.nlse = stats;
   a.delta = stats + (size_t)Hq * T;
-  a.start = start; a.end = end; a.meta = meta;
+  a.start = start; a.end = end; a.meta = meta; a.order = order;
   a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo; a.lddo = lddo; a.ldout = lddq; a.lddk = lddk; a.lddv = lddv;
   a.T = T; a.Hq = Hq; a.Hkv = Hkv;
   a.c = scale * 1.4426950408889634f;
   a.scale = scale;
   a.fill = fill;
-  a.nsplit = D == 128 ? key_splits(T, Hkv) : 1;
+  a.nsplit = key_splits(T, Hkv, D);
   a.part = part;
   if (a.nsplit > 1 && (!part || ((uintptr_t)part & 15) || part_floats < mx_packed_attn_bwd_floats(T, Hkv, D)))
     return hipErrorInvalidValue;
   const unsigned nb = (unsigned)((T + 127) / 128);
   if (D == 64) {
     hipLaunchKernelGGL((packed_qmajor_kernel<64, true>), dim3(nb * Hq), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((packed_kmajor_kernel<64>), dim3(nb * Hkv), dim3(256), 0, s, a);
+    a.order = order + nb;
+    hipLaunchKernelGGL((packed_kmajor_kernel<64>), dim3(nb * Hkv * a.nsplit), dim3(256), 0, s, a);
   } else {
     hipLaunchKernelGGL((packed_qmajor_kernel<128, true>), dim3(nb * Hq), dim3(256), 0, s, a);
     const unsigned nk = (unsigned)((T + KB2 - 1) / KB2);
+    a.order = order + 2 * nb;
     hipLaunchKernelGGL((packed_kmajor2_kernel<128>), dim3(nk * Hkv * a.nsplit), dim3(256), 0, s, a);
-    if (a.nsplit > 1) {
-      const int64_t vecs = (int64_t)T * Hkv * 32;
-      hipLaunchKernelGGL((packed_join_kernel<128>), dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, s, a);
-    }
+  }
+  if (a.nsplit > 1) {
+    const dim3 grid((unsigned)(((int64_t)T * Hkv * (D / 4) + 255) / 256));
+    if (D == 64) hipLaunchKernelGGL((packed_join_kernel<64>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((packed_join_kernel<128>), grid, dim3(256), 0, s, a);
   }
   return hipGetLastError();
 }

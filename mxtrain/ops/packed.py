@@ -27,12 +27,13 @@ class PackedSequences:
     the bounds of its sequence (``start``, ``end``, int32) and its position in it
     (``positions``, int64: RoPE's ``pos_ids``, the rows of a learned position table)."""
 
-    __slots__ = ("cu_seqlens", "total", "start", "end", "meta", "positions", "ptrs")
+    __slots__ = ("cu_seqlens", "total", "start", "end", "meta", "positions", "order", "ptrs")
 
-    def __init__(self, cu_seqlens, total, start, end, meta, positions):
-        self.cu_seqlens, self.total = cu_seqlens, total
+    def __init__(self, cu_seqlens, total, start, end, meta, positions, order=None):
+        self.cu_seqlens, self.total, self.order = cu_seqlens, total, order
         self.start, self.end, self.meta, self.positions = start, end, meta, positions
-        self.ptrs = (start.data_ptr(), end.data_ptr(), meta.data_ptr())   # (this object owns the tensors)
+        # kernel arguments (this object owns the tensors)
+        self.ptrs = (start.data_ptr(), end.data_ptr(), meta.data_ptr(), _lib.ptr(order))
 
     @property
     def device(self):
@@ -69,12 +70,13 @@ def pack_sequences(cu_seqlens: torch.Tensor, total: int, device=None) -> PackedS
         meta = torch.tensor([nv, 0, 0, 0], dtype=torch.int32, device=dev)
         return PackedSequences(cu, total, start.int(), end.int(), meta, t - start)
     with _lib.on_device(cu):
-        tab = torch.empty(2 * total + 4, dtype=torch.int32, device=cu.device)
+        tab = torch.empty(2 * total + 4 + _lib.query64("mx_packed_order_len", total), dtype=torch.int32,
+                          device=cu.device)
         pos = torch.empty(total, dtype=torch.int64, device=cu.device)
-        start, end, meta = tab[:total], tab[total:2 * total], tab[2 * total:]
+        start, end, meta, order = tab.split((total, total, 4, tab.numel() - 2 * total - 4))
         _lib.call("mx_packed_plan", _lib.ptr(cu), int(cu.dtype == torch.int64), n, total, _lib.ptr(start),
-                  _lib.ptr(end), _lib.ptr(meta), _lib.ptr(pos), _lib.stream())
-    return PackedSequences(cu, total, start, end, meta, pos)
+                  _lib.ptr(end), _lib.ptr(meta), _lib.ptr(pos), _lib.ptr(order), _lib.stream())
+    return PackedSequences(cu, total, start, end, meta, pos, order)
 
 
 # ------------------------------------------------------------------ checks

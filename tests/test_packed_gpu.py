@@ -247,3 +247,23 @@ def test_captured_step_replays_on_new_batches():
         got = [t.clone() for t in outs]
         for x, y in zip(got, go()):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_non_finite_values_beside_split_key_blocks(D):
+    """Few key heads and long sequences: key blocks split over workgroups, with NaN next door."""
+    lens, Hq, Hkv = [1300, 900], 4, 1
+    T = sum(lens) + 10
+    q, k, v, do = _inputs(T, Hq, Hkv, D, seed=21)
+    s = ops.pack_sequences(_cu(lens), T, device=DEV)
+    want = attention(q, k, v, lens, Hq, Hkv, D, D ** -0.5, do)
+    for t in (q, k, v, do):
+        t[1290:1300] = float("nan")
+        t[2200:] = float("inf")
+    o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D)
+    grads = ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D)
+    for name, t in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+        within(t[1300:2200], tuple(x[1300:2200] for x in want[name]), name)
+        assert (t[2200:] == 0).all(), name
+    within(o[:1290], tuple(x[:1290] for x in want["o"]), "o")
+    assert torch.isnan(o[1290:1300]).all() and torch.isnan(grads[1][:1300]).all()
