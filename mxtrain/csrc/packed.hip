@@ -62,24 +62,32 @@ __global__ __launch_bounds__(256) void packed_plan_kernel(const IT* __restrict__
 // Dispatch order of the 128-row query blocks, the 128-key and the 256-key blocks: most work first
 // (ties: query blocks from the back, key blocks from the front), so that the longest blocks of a batch
 // of mixed lengths do not start last.  One workgroup counts each block's rank; order: [nq][nk][nk2].
-// Above ORDER_MAX blocks the lists are left in sequence order.
+// Above ORDER_MAX blocks the lists are left in sequence order.  meta[1], meta[2]: query tiles of all
+// 128- / 256-key blocks (how much a split key block should hold).
 constexpr int ORDER_MAX = 2048;
 __global__ __launch_bounds__(1024) void packed_order_kernel(int T, const int* __restrict__ start,
-                                                            const int* __restrict__ end, const int* __restrict__ meta,
+                                                            const int* __restrict__ end, int* __restrict__ meta,
                                                             int* __restrict__ order) {
   __shared__ int work[ORDER_MAX];
+  __shared__ int sum[3];
   const int nv = meta[0], tid = threadIdx.x;
+  if (tid < 3) sum[tid] = 0;
+  __syncthreads();
 #pragma unroll 1
   for (int list = 0; list < 3; ++list) {
     const int B = list == 2 ? 256 : 128, nb = (T + B - 1) / B;
-    if (nb > ORDER_MAX) {
-      for (int b = tid; b < nb; b += 1024) order[b] = list == 0 ? nb - 1 - b : b;
-    } else {
-      for (int b = tid; b < nb; b += 1024) {
-        const int b0 = b * B, b1 = min(b0 + B, nv);
-        work[b] = b0 >= nv ? 0 : list == 0 ? b1 - start[b0] : end[b1 - 1] - b0;
-      }
-      __syncthreads();
+    int tiles = 0;
+    for (int b = tid; b < nb; b += 1024) {
+      const int b0 = b * B, b1 = min(b0 + B, nv);
+      const int w = b0 >= nv ? 0 : list == 0 ? b1 - start[b0] : end[b1 - 1] - b0;
+      tiles += (w + 63) / 64;
+      if (nb <= ORDER_MAX) work[b] = w;
+      else order[b] = list == 0 ? nb - 1 - b : b;
+    }
+    atomicAdd(&sum[list], tiles);
+    __syncthreads();
+    if (list > 0 && tid == 0) meta[list] = sum[list];
+    if (nb <= ORDER_MAX) {
       for (int b = tid; b < nb; b += 1024) {
         const int w = work[b];
         int rank = 0;
@@ -88,8 +96,8 @@ __global__ __launch_bounds__(1024) void packed_order_kernel(int T, const int* __
           rank += (int)(work[o] > w) | ((int)(work[o] == w) & (int)(list == 0 ? o > b : o < b));
         order[rank] = b;
       }
-      __syncthreads();
     }
+    __syncthreads();
     order += nb;
   }
 }
@@ -485,8 +493,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
 // ============================================================================ key-major
 constexpr int KB1 = 128, KB2 = 256, QT2 = 64;   // keys of a block (D = 64 / 128), rows of a query tile
-constexpr int SPLIT_MIN = 24;                   // fewest items of a split
-__device__ __forceinline__ int block_splits(int items, int nsplit) { return max(1, min(nsplit, items / SPLIT_MIN)); }
+// Splits of a key block of `items` (query head, query tile) pairs: a split holds a workgroup slot's even
+// share of the batch (meta: the query tiles of all blocks of one head) and a few items more, which pay
+// for its partial sums.  dQ, dK, dV of 8 query heads on one key head, 512 tokens: 73 -> 38 us (D 64),
+// 156 -> 65 us (D 128); without the extra items 4096 tokens of ~300-token documents take 120 us, not 99
+// (16 heads of 128); with shares twice as large 16384 tokens, 16 / 4 heads, take 4.9 ms, not 3.8.
+template <int D>
+__device__ __forceinline__ int block_splits(const PArgs& a, int items) {
+  const int64_t even = (int64_t)a.meta[D == 64 ? 1 : 2] * a.Hq / (D == 64 ? 512 : 256);
+  const int share = (int)min(even, (int64_t)1 << 30) + 5;
+  return max(1, min(a.nsplit, (items + share - 1) / share));
+}
 
 // Where a key block's dK / dV go: the results, or fp32 partials of its split [split][dk, dv][T][Hkv D]
 template <int D>
@@ -603,7 +620,7 @@ packed_kmajor_kernel(const PArgs a) {
     return;
   }
   const int nqt = (qend - k0 + QT - 1) / QT, items = nqt * grp;
-  const int nsp = block_splits(items, a.nsplit), per = (items + nsp - 1) / nsp;
+  const int nsp = uni(block_splits<D>(a, items)), per = (items + nsp - 1) / nsp;
   const int t0 = sp * per, t1 = min(items, t0 + per);
   if (sp >= nsp) return;
   const bool wave_on = kw < nv;
@@ -796,7 +813,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     return;
   }
   const int nqt = (qend - k0 + QT - 1) / QT, items = nqt * grp;
-  const int nsp = block_splits(items, a.nsplit), per = (items + nsp - 1) / nsp;
+  const int nsp = uni(block_splits<D>(a, items)), per = (items + nsp - 1) / nsp;
   const int t0 = sp * per, t1 = min(items, t0 + per);
   if (sp >= nsp) return;
   const bool wave_on = kw < nv;
@@ -1024,7 +1041,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PArgs a) {
   constexpr int KB = D == 64 ? KB1 : KB2;
   const int col = (int)(v - t * nw) * 4, k0 = (int)t / KB * KB;
   const int nqt = (min(a.end[min(k0 + KB, a.T) - 1], nv) - k0 + QT2 - 1) / QT2;
-  const int nsp = block_splits(nqt * (a.Hq / a.Hkv), a.nsplit);
+  const int nsp = block_splits<D>(a, nqt * (a.Hq / a.Hkv));
   if (nsp == 1) return;
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
@@ -1039,12 +1056,14 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PArgs a) {
   }
 }
 
-// splits of the key blocks: enough workgroups for several rounds of the chip
-int key_splits(int T, int Hkv, int D) {
+// most splits of a key block: until there are 1024 workgroups, or 512 where a key head has one query
+// head (4096 tokens of ~300-token documents, 16 / 16 heads of 64: 53 us unsplit, 60 in two; 16 / 4 heads,
+// 16384 tokens: 472 and 352)
+int key_splits(int T, int Hq, int Hkv, int D) {
   const int kb = D == 64 ? KB1 : KB2;
   const int64_t blocks = (int64_t)((T + kb - 1) / kb) * Hkv;
   int n = 1;
-  while (n < (D == 64 ? 8 : 4) && blocks * n < (D == 64 ? 512 : 1024)) n *= 2;
+  while (n < 16 && blocks * n < (Hq > Hkv ? 1024 : 512)) n *= 2;
   return n;
 }
 
@@ -1102,9 +1121,9 @@ MX_EXPORT int mx_packed_attn_fwd(const void* q, const void* k, const void* v, in
 }
 
 // floats of `part` (0: none)
-MX_EXPORT int64_t mx_packed_attn_bwd_floats(int T, int Hkv, int D) {
-  if (T <= 0 || Hkv <= 0 || (D != 64 && D != 128)) return 0;
-  const int n = key_splits(T, Hkv, D);
+MX_EXPORT int64_t mx_packed_attn_bwd_floats(int T, int Hq, int Hkv, int D) {
+  if (T <= 0 || Hq <= 0 || Hkv <= 0 || (D != 64 && D != 128)) return 0;
+  const int n = key_splits(T, Hq, Hkv, D);
   return n > 1 ? (int64_t)n * 2 * T * Hkv * D : 0;
 }
 
@@ -1132,9 +1151,9 @@ MX_EXPORT int mx_packed_attn_bwd(const void* q, const void* k, const void* v, in
   a.c = scale * 1.4426950408889634f;
   a.scale = scale;
   a.fill = fill;
-  a.nsplit = key_splits(T, Hkv, D);
+  a.nsplit = key_splits(T, Hq, Hkv, D);
   a.part = part;
-  if (a.nsplit > 1 && (!part || ((uintptr_t)part & 15) || part_floats < mx_packed_attn_bwd_floats(T, Hkv, D)))
+  if (a.nsplit > 1 && (!part || ((uintptr_t)part & 15) || part_floats < mx_packed_attn_bwd_floats(T, Hq, Hkv, D)))
     return hipErrorInvalidValue;
   const unsigned nb = (unsigned)((T + 127) / 128);
   if (D == 64) {

@@ -235,7 +235,7 @@ def packed_attn_bwd(dout, q, k, v, o, lse, seqs: PackedSequences, Hq: int, Hkv: 
             dv = torch.empty(T, Hkv * D, dtype=q.dtype, device=q.device)
             grads = (dq.data_ptr(), Hq * D), (dk.data_ptr(), Hkv * D), (dv.data_ptr(), Hkv * D)
         stats = torch.empty(2, Hq, T, dtype=torch.float32, device=q.device)
-        nf = _lib.query64("mx_packed_attn_bwd_floats", T, Hkv, D)
+        nf = _lib.query64("mx_packed_attn_bwd_floats", T, Hq, Hkv, D)
         part = torch.empty(nf, dtype=torch.float32, device=q.device) if nf else None
         (dq_, lddq), (dk_, lddk), (dv_, lddv) = grads
         _lib.call("mx_packed_attn_bwd", q_, k_, v_, ldq, ldk, ldv, o_, ldo, do_, lddo, lse.data_ptr(),
