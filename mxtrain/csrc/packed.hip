@@ -61,18 +61,22 @@ __global__ __launch_bounds__(256) void packed_plan_kernel(const IT* __restrict__
 
 // Dispatch order of the 128-row query blocks, the 128-key and the 256-key blocks: most work first
 // (ties: query blocks from the back, key blocks from the front), so that the longest blocks of a batch
-// of mixed lengths do not start last.  One workgroup counts each block's rank; order: [nq][nk][nk2].
-// Above ORDER_MAX blocks the lists are left in sequence order.  meta[1], meta[2]: query tiles of all
-// 128- / 256-key blocks (how much a split key block should hold).
+// of mixed lengths do not start last.  One workgroup counts each block's rank; above ORDER_MAX blocks
+// the lists are left in sequence order.  meta[1]: query tiles of all 128-key blocks (how much a split
+// key block should hold).  Behind the lists (order_base), the query tiles of all 256-key blocks before
+// each, which the D = 128 dK / dV kernel cuts into shares.
 constexpr int ORDER_MAX = 2048;
+__host__ __device__ inline int64_t order_base(int T) { return (2 * ((int64_t)(T + 127) / 128) + (T + 255) / 256 + 1) & ~1ll; }
 __global__ __launch_bounds__(1024) void packed_order_kernel(int T, const int* __restrict__ start,
                                                             const int* __restrict__ end, int* __restrict__ meta,
                                                             int* __restrict__ order) {
   __shared__ int work[ORDER_MAX];
-  __shared__ int sum[3];
+  __shared__ int sum;
+  __shared__ int64_t scan[2][1024];
   const int nv = meta[0], tid = threadIdx.x;
-  if (tid < 3) sum[tid] = 0;
+  if (tid == 0) sum = 0;
   __syncthreads();
+  int* list0 = order;
 #pragma unroll 1
   for (int list = 0; list < 3; ++list) {
     const int B = list == 2 ? 256 : 128, nb = (T + B - 1) / B;
@@ -84,9 +88,9 @@ __global__ __launch_bounds__(1024) void packed_order_kernel(int T, const int* __
       if (nb <= ORDER_MAX) work[b] = w;
       else order[b] = list == 0 ? nb - 1 - b : b;
     }
-    atomicAdd(&sum[list], tiles);
+    if (list == 1) atomicAdd(&sum, tiles);
     __syncthreads();
-    if (list > 0 && tid == 0) meta[list] = sum[list];
+    if (list == 1 && tid == 0) meta[1] = sum;
     if (nb <= ORDER_MAX) {
       for (int b = tid; b < nb; b += 1024) {
         const int w = work[b];
@@ -100,6 +104,26 @@ __global__ __launch_bounds__(1024) void packed_order_kernel(int T, const int* __
     __syncthreads();
     order += nb;
   }
+  int64_t* before = reinterpret_cast<int64_t*>(list0 + order_base(T));
+  const int nb2 = (T + 255) / 256;
+  int64_t base = 0;
+#pragma unroll 1
+  for (int c0 = 0; c0 < nb2; c0 += 1024) {
+    const int b0 = (c0 + tid) * 256;
+    int64_t x = c0 + tid < nb2 && b0 < nv ? (end[min(b0 + 256, nv) - 1] - b0 + 63) / 64 : 0;
+    scan[0][tid] = x;
+    __syncthreads();
+    int p = 0;
+#pragma unroll 1
+    for (int d = 1; d < 1024; d *= 2, p ^= 1) {
+      scan[p ^ 1][tid] = scan[p][tid] + (tid >= d ? scan[p][tid - d] : 0);
+      __syncthreads();
+    }
+    if (c0 + tid < nb2) before[c0 + tid + 1] = base + scan[p][tid];
+    base += scan[p][1023];
+    __syncthreads();
+  }
+  if (tid == 0) before[0] = 0;
 }
 
 struct PArgs {
@@ -112,7 +136,9 @@ struct PArgs {
   int T, Hq, Hkv;
   float c, scale;               // scale log2(e), scale
   float* part;                  // partial dK / dV of split blocks
-  int nsplit;
+  int nsplit;                   // most splits of a key block
+  int nshare;                   // most shares (see KeyShare; 0: blocks are split by themselves)
+  const int64_t* before;        // query tiles of the 256-key blocks before each
   int fill;                     // zero the rows behind the last sequence (else leave them)
 };
 
@@ -500,31 +526,76 @@ constexpr int KB1 = 128, KB2 = 256, QT2 = 64;   // keys of a block (D = 64 / 128
 // (16 heads of 128); with shares twice as large 16384 tokens, 16 / 4 heads, take 4.9 ms, not 3.8.
 template <int D>
 __device__ __forceinline__ int block_splits(const PArgs& a, int items) {
-  const int64_t even = (int64_t)a.meta[D == 64 ? 1 : 2] * a.Hq / (D == 64 ? 512 : 256);
+  const int64_t even = (D == 64 ? (int64_t)a.meta[1] : a.before[(a.T + KB2 - 1) / KB2]) * a.Hq / (D == 64 ? 512 : 256);
   const int share = (int)min(even, (int64_t)1 << 30) + 5;
   return max(1, min(a.nsplit, (items + share - 1) / share));
 }
 
-// Where a key block's dK / dV go: the results, or fp32 partials of its split [split][dk, dv][T][Hkv D]
+// D = 128, few key blocks: the items of all of them, head by head and block by block, are one line that
+// is cut into even shares, one per workgroup; a block that a cut falls into is done in pieces, whose
+// fp32 sums packed_join2_kernel adds.  A block costs PIECE items beside its own (its K and V rows, its
+// results), a piece about SNAP (its partial sums): a cut nearer to the end of a block moves there.
+constexpr int PIECE = 2, SNAP = 5, SHARE_MIN = 8;
+__device__ __forceinline__ int64_t uni64(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)uni((int)x) | (uint64_t)(uint32_t)uni((int)(x >> 32)) << 32);
+}
+struct KeyShare {
+  const int64_t* before;    // query tiles of the blocks before each
+  int nb, grp, n;           // blocks, query heads of a key head, shares
+  int64_t head, total;      // length of a head's line, of all
+  __device__ __forceinline__ KeyShare(const PArgs& a, int nv)
+      : before(a.before), nb((nv + KB2 - 1) / KB2), grp(a.Hq / a.Hkv) {
+    head = off(nb);
+    total = head * a.Hkv;
+    n = (int)min((int64_t)a.nshare, (total + SHARE_MIN - 1) / SHARE_MIN);
+  }
+  struct Pos { int64_t line; int hk, blk; int64_t f; };    // on the line; head, block, offset in the block
+  __device__ __forceinline__ int64_t off(int b) const { return grp * before[b] + PIECE * (int64_t)b; }
+  // where share w begins; a wave probes 64 blocks at a time
+  __device__ __forceinline__ Pos first(int w, int lane) const {
+    Pos p;
+    p.line = total * w / n;
+    p.hk = uni((int)(p.line / head));
+    const int64_t q = p.line - p.hk * head;
+    int lo = 0, cnt = nb;
+    while (cnt > 1) {
+      const int step = (cnt + 63) / 64, x = lane * step;
+      const int k = __popcll(__ballot(x < cnt && off(lo + min(x, cnt - 1)) <= q)) - 1;
+      lo += k * step;
+      cnt = min(step, cnt - k * step);
+    }
+    p.blk = uni(lo);
+    p.f = q - off(lo);
+    if (w == n) return p;                                  // (the end of the line: never looked into)
+    const int64_t left = off(lo + 1) - q;
+    if (p.f <= PIECE + SNAP) {
+      p.line -= p.f;
+      p.f = 0;
+    } else if (left <= SNAP) {
+      p.line += left;
+      p.f = 0;
+      if (++p.blk == nb) { p.blk = 0; ++p.hk; }
+    }
+    return p;
+  }
+};
+
+// Where a key block's dK / dV go: the results, or (pk given) fp32 partial sums, key row0 first, W floats a row
 template <int D>
 struct KeyOut {
   const PArgs& a;
-  int hk, nsp, lane, W;
+  int hk, lane;
   float *pk, *pv;
-  __device__ __forceinline__ KeyOut(const PArgs& a_, int hk_, int sp, int nsp_, int lane_)
-      : a(a_), hk(hk_), nsp(nsp_), lane(lane_), W(a_.Hkv * D) {
-    pk = a.part + (size_t)sp * 2 * a.T * W + hk * D;
-    pv = pk + (size_t)a.T * W;
-  }
+  int row0, W;
   // the accumulators of one key per lane pair
   template <int N>
   __device__ __forceinline__ void put(int key, const f32x16 (&dk)[N], const f32x16 (&dv)[N], int hh) const {
-    if (nsp > 1) {
+    if (pk) {
 #pragma unroll
       for (int dt = 0; dt < N; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-          const size_t o = (size_t)key * W + 32 * dt + 2 * e + 4 * hh;
+          const size_t o = (size_t)(key - row0) * W + 32 * dt + 2 * e + 4 * hh;
           *reinterpret_cast<float4*>(pk + o) = make_float4(dk[dt][e], dk[dt][e + 1], dk[dt][e + 2], dk[dt][e + 3]);
           *reinterpret_cast<float4*>(pv + o) = make_float4(dv[dt][e], dv[dt][e + 1], dv[dt][e + 2], dv[dt][e + 3]);
         }
@@ -537,11 +608,11 @@ struct KeyOut {
     }
   }
   __device__ __forceinline__ void put(int key, const RowVec<D>& dk, const RowVec<D>& dv) const {
-    if (nsp > 1) {
+    if (pk) {
 #pragma unroll
       for (int x = 0; x < D / 64; ++x) {
-        pk[(size_t)key * W + lane + 64 * x] = dk.x[x];
-        pv[(size_t)key * W + lane + 64 * x] = dv.x[x];
+        pk[(size_t)(key - row0) * W + lane + 64 * x] = dk.x[x];
+        pv[(size_t)(key - row0) * W + lane + 64 * x] = dv.x[x];
       }
       return;
     }
@@ -580,7 +651,7 @@ __device__ __forceinline__ void redo_keys(const PArgs& a, const KeyOut<D>& out, 
 // dK, dV: key on the MFMA lane; Q / dO tiles of QT rows (and their statistics) stream through a
 // two-slot LDS-DMA ring, over the query heads of the key head's group.  Where there are few key blocks,
 // those of long sequences are split along their (query head, query tile) items over up to `nsplit`
-// workgroups, whose fp32 partial sums packed_join_kernel adds in order.
+// workgroups, whose fp32 partial sums packed_join_kernel adds in order (or all are cut, see KeyShare).
 //
 // D = 64.  Four waves of 32 keys, two waves per SIMD.
 template <int D>
@@ -752,7 +823,9 @@ packed_kmajor_kernel(const PArgs a) {
     zero_row<D>(dkp, hh);
     zero_row<D>(dvp, hh);
   }
-  const KeyOut<D> out(a, hk, sp, nsp, lane);
+  const int W = a.Hkv * D;                             // partials: [split][dk, dv][T][Hkv D]
+  float* pk = nsp > 1 ? a.part + (size_t)sp * 2 * T * W + hk * D : nullptr;
+  const KeyOut<D> out{a, hk, lane, pk, pk + (size_t)T * W, 0, W};
   if (__any(bad != 0)) {
     redo_keys<D>(a, out, kw, min(kw + 31, nv - 1), k0, t0, t1, nqt, hk, grp, lane);
     return;
@@ -778,25 +851,73 @@ __device__ __forceinline__ void mfma_v_done(f32x16& a, f32x16& b) {
   asm volatile("s_nop 15\n\ts_nop 7" : "+v"(a), "+v"(b));
 }
 
-template <int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void packed_kmajor2_kernel(const PArgs a) {
+template <int D, bool SHARES>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void packed_kmajor2_kernel(const PArgs a0) {
   constexpr int NL = 4;   // the V fragments of odd kk stay in LDS: the registers do not hold all
   constexpr int QT = QT2, NQS = QT / 32, NKK = D / 16, NDT = D / 32;
   constexpr int RB = D * 2, CPR = D / 8, RPP = 64 / CPR, TILE = QT * RB, PPW = TILE / 1024 / 4;
   __shared__ __attribute__((aligned(16))) char ring[2][2 * TILE];   // Q, dO
   __shared__ __attribute__((aligned(16))) float stat[2][2][64];     // -lse / c, -delta
   __shared__ __attribute__((aligned(16))) uint4 vlds[4][2 * NL][64];  // the waves' V fragments of odd kk
-  const int tid = threadIdx.x, lane = tid & 63, wl = uni(tid >> 6);
-  const int r = lane & 31, hh = lane >> 5, g = lane >> 4, gi = lane & 15;
-  const int T = a.T;
-  const int nblk = gridDim.x / a.nsplit, sp = blockIdx.x / nblk;
-  int rank, hk;
-  block_map(blockIdx.x - sp * nblk, a.Hkv, rank, hk);
-  const int grp = a.Hq / a.Hkv;
-  const int k0 = uni(a.order[rank]) * KB2, kw = k0 + 64 * wl;
-  const int nv = uni(a.meta[0]);
+  const int lane0 = threadIdx.x & 63, wl = uni((int)threadIdx.x >> 6);
+  const int nv = uni(a0.meta[0]);
+  if (a0.fill)                                          // rows behind the last sequence
+    for (int64_t x = (int64_t)nv * a0.Hkv + blockIdx.x * 4 + wl; x < (int64_t)a0.T * a0.Hkv; x += gridDim.x * 4) {
+      const int64_t row = x / a0.Hkv;
+      const int col = (int)(x - row * a0.Hkv) * D + 2 * lane0;
+      *reinterpret_cast<uint32_t*>(a0.dk + row * a0.lddk + col) = 0;
+      *reinterpret_cast<uint32_t*>(a0.dv + row * a0.lddv + col) = 0;
+    }
+  const int nbv = (nv + KB2 - 1) / KB2;                // blocks with work
+  int w = 0, hk, blk, sp = 0;
+  int64_t f = 0, left = 0;                             // offset in the block; what is left of the share
+  if constexpr (SHARES) {                              // a share to each workgroup, neighbours on one XCD
+    const KeyShare ks(a0, nv);
+    if ((int)blockIdx.x >= ks.n) return;
+    const int n8 = ks.n >> 3, x = (int)blockIdx.x;
+    w = x < 8 * n8 ? (x & 7) * n8 + (x >> 3) : x;
+    const KeyShare::Pos p = ks.first(w, lane0);
+    hk = uni(p.hk); blk = uni(p.blk); f = uni64(p.f);
+    left = uni64(ks.first(w + 1, lane0).line - p.line);
+    if (left <= 0) return;
+  } else {                                             // a block, or a split of it, to each
+    const int nblk = gridDim.x / a0.nsplit;
+    sp = blockIdx.x / nblk;
+    block_map(blockIdx.x - sp * nblk, a0.Hkv, blk, hk);
+    blk = uni(a0.order[blk]);
+    if (blk >= nbv) return;
+  }
+#pragma unroll 1
+  for (;; blk + 1 < nbv ? ++blk : (blk = 0, ++hk)) {
+  // (the arguments are read again for every block: kept across blocks they and what derives from them
+  // overflow the scalar registers, and those they spill to)
+  const PArgs& a = a0;
+  const int T = a.T, grp = a.Hq / a.Hkv;
+  const int k0 = blk * KB2, kw = k0 + 64 * wl;
   const int qend = min(uni(a.end[min(k0 + KB2, T) - 1]), nv);
   const int emax = min(uni(a.end[min(kw + 63, T - 1)]), nv);
+  const int nqt = (qend - k0 + QT - 1) / QT, items = nqt * grp;
+  int t0, t1, nsp = 1;
+  if constexpr (SHARES) {
+    const int64_t take = min(left, items + PIECE - f);
+    t0 = uni((int)max(f - PIECE, (int64_t)0));
+    t1 = uni((int)(f + take - PIECE));
+    left -= take;
+    f = 0;
+    if (t1 <= t0) {
+      if (left <= 0) break;
+      continue;
+    }
+  } else {
+    nsp = uni(block_splits<D>(a, items));
+    const int per = (items + nsp - 1) / nsp;
+    t0 = sp * per;
+    t1 = min(items, t0 + per);
+    if (sp >= nsp) return;
+  }
+  int lane = lane0;                                    // (no table of it is kept across blocks: there are no registers)
+  asm volatile("" : "+v"(lane));
+  const int r = lane & 31, hh = lane >> 5, g = lane >> 4, gi = lane & 15;
   int key[2], cnt[2], emin[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -804,18 +925,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     cnt[j] = a.end[min(key[j], T - 1)] - key[j];       // rows that see this key: key .. key + cnt - 1
     emin[j] = uni(a.end[min(kw + 32 * j, T - 1)]);
   }
-  if (k0 >= nv) {
-    if (a.fill && sp == 0)
-      for (int key = kw + r; key < min(kw + 64, T); key += 32) {
-        zero_row<D>(a.dk + (size_t)key * a.lddk + hk * D, hh);
-        zero_row<D>(a.dv + (size_t)key * a.lddv + hk * D, hh);
-      }
-    return;
-  }
-  const int nqt = (qend - k0 + QT - 1) / QT, items = nqt * grp;
-  const int nsp = uni(block_splits<D>(a, items)), per = (items + nsp - 1) / nsp;
-  const int t0 = sp * per, t1 = min(items, t0 + per);
-  if (sp >= nsp) return;
   const bool wave_on = kw < nv;
   const int klast = min(kw + 63, nv - 1);
   uint32_t bad = 0;   // (see packed_qmajor_kernel)
@@ -1014,19 +1123,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     if (uni(wave_on && qs < emax && qs + QT > kw ? 1 : 0))
       body(ring[slot], ring[slot] + TILE, stat[slot][0], stat[slot][1], qs);
   }
-  const KeyOut<D> out(a, hk, sp, nsp, lane);
+  const int W = SHARES ? D : a.Hkv * D;                // partials: of a piece [dk, dv][KB2][D], or as of D = 64
+  float *pk = nullptr, *pv = nullptr;
+  if (SHARES ? t1 - t0 < items : nsp > 1) {
+    pk = a.part + (SHARES ? (size_t)(2 * w + (t0 == 0 ? 1 : 0)) * 2 * KB2 * D : (size_t)sp * 2 * T * W + hk * D);
+    pv = pk + (size_t)(SHARES ? KB2 : T) * W;
+  }
+  const KeyOut<D> out{a, hk, lane, pk, pv, SHARES ? k0 : 0, W};
   const bool redo = __any(bad != 0);
   if (redo) redo_keys<D>(a, out, kw, klast, k0, t0, t1, nqt, hk, grp, lane);
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    if (key[j] >= nv) {
-      if (a.fill && sp == 0 && key[j] < T) {
-        zero_row<D>(a.dk + (size_t)key[j] * a.lddk + hk * D, hh);
-        zero_row<D>(a.dv + (size_t)key[j] * a.lddv + hk * D, hh);
-      }
-    } else if (!redo) {
-      out.put(key[j], dkacc[j], dvacc[j], hh);
-    }
+  for (int j = 0; j < 2; ++j)
+    if (key[j] < nv && !redo) out.put(key[j], dkacc[j], dvacc[j], hh);
+  if (!SHARES || left <= 0) break;
+  __syncthreads();                                     // the ring is free for the next block
   }
 }
 
@@ -1056,6 +1166,37 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PArgs a) {
   }
 }
 
+// D = 128: the blocks that the ends of shares cut.  JOIN workgroups for the end of each share w; the one
+// where the cut block's first piece ends adds all of its pieces, in the order of the shares.
+constexpr int JOIN = 16;
+__global__ __launch_bounds__(256) void packed_join2_kernel(const PArgs a) {
+  constexpr int D = 128;
+  const int w = blockIdx.x / JOIN, lane = threadIdx.x & 63, nv = uni(a.meta[0]);
+  const KeyShare ks(a, nv);
+  if (w + 1 >= ks.n) return;
+  const KeyShare::Pos cut = ks.first(w + 1, lane);
+  if (cut.f == 0) return;                              // between two blocks
+  const int64_t b0 = cut.line - cut.f;                 // the block's first item is of share w, or of one before
+  if (ks.first(w, lane).line > b0) return;
+  const int64_t b1 = b0 + ks.off(cut.blk + 1) - ks.off(cut.blk);
+  int last = w + 1;
+  while (last + 1 < ks.n && ks.first(last + 1, lane).line < b1) ++last;
+  const int hk = cut.hk, blk = cut.blk;
+  const int k0 = blk * KB2, n = min(KB2, nv - k0) * (D / 4);
+  for (int x = (blockIdx.x % JOIN) * 256 + threadIdx.x; x < 2 * n; x += JOIN * 256) {
+    const int which = x >= n, y = x - which * n, row = k0 + y / (D / 4), col = hk * D + y % (D / 4) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = w; k <= last; ++k) {
+      const float* p = a.part + (size_t)((2 * k + (k == w ? 1 : 0)) * 2 + which) * KB2 * D + 4 * (size_t)y;
+      const float4 v = *reinterpret_cast<const float4*>(p);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    const float sc = which ? 1.f : a.scale;
+    uint16_t* o = which ? a.dv + (size_t)row * a.lddv : a.dk + (size_t)row * a.lddk;
+    *reinterpret_cast<uint2*>(o + col) = make_uint2(pack2(s.x * sc, s.y * sc), pack2(s.z * sc, s.w * sc));
+  }
+}
+
 // most splits of a key block: until there are 1024 workgroups, or 512 where a key head has one query
 // head (4096 tokens of ~300-token documents, 16 / 16 heads of 64: 53 us unsplit, 60 in two; 16 / 4 heads,
 // 16384 tokens: 472 and 352)
@@ -1066,13 +1207,22 @@ int key_splits(int T, int Hq, int Hkv, int D) {
   while (n < 16 && blocks * n < (Hq > Hkv ? 1024 : 512)) n *= 2;
   return n;
 }
+// Most shares, one per CU, or 0: shared heads of D = 128 have few key blocks, and shares beat splits
+// once there is work enough to pay for the joining, unless there are blocks enough to keep the CUs
+// evenly busy.  dQ, dK, dV in us by shares and by splits: 8001 tokens of ~900-token documents, 32 / 8
+// heads, 410 and 465; 16384 of ~1000, 8 / 1 heads, 295 and 412; 4096 in one, 16 / 4 heads, 320 and 390;
+// but 4096 of ~300, 8 / 1 heads, 121 and 90; 512 in one 106 and 62; own heads, 8001 of ~900, 270 and 240.
+int key_shares(int T, int Hq, int Hkv, int D) {
+  const int64_t blocks = (int64_t)((T + KB2 - 1) / KB2) * Hkv;
+  return D == 128 && Hq > Hkv && blocks < 1024 && (int64_t)T * Hq >= 60000 ? 256 : 0;
+}
 
 bool bad_mat(const void* p, int ld, int width) {   // 16-B rows, tile offsets below 2^31 bytes
   return p == nullptr || ((uintptr_t)p & 15) || (ld & 7) || ld < width || ld > (1 << 22);
 }
 bool bad_shape(int T, int Hq, int Hkv, int D) {
   if (T <= 0 || T > (1 << 30) || Hq <= 0 || Hkv <= 0 || Hq % Hkv || (D != 64 && D != 128)) return true;
-  return (int64_t)((T + 127) / 128) * Hq >= ((int64_t)1 << 31);
+  return (int64_t)((T + 127) / 128) * Hq >= ((int64_t)1 << 31) || (int64_t)((T + 63) / 64) * (Hq / Hkv) >= 1 << 30;
 }
 
 }  // namespace
@@ -1094,7 +1244,7 @@ MX_EXPORT int mx_packed_plan(const void* cu, int wide, int n, int T, int* start,
 }
 
 // int32 entries of `order` for T rows
-MX_EXPORT int64_t mx_packed_order_len(int T) { return T > 0 ? 2 * ((int64_t)(T + 127) / 128) + (T + 255) / 256 : 0; }
+MX_EXPORT int64_t mx_packed_order_len(int T) { return T > 0 ? order_base(T) + 2 * ((T + 255) / 256 + 1) : 0; }
 
 // Q, K, V, O: bf16 [T] rows with strides ld*, head h at column h D.  lse: fp32 [Hq][T], base 2.
 // fill: rows behind the last sequence get o = 0, lse = +inf; else they are left as they are.
@@ -1122,7 +1272,8 @@ MX_EXPORT int mx_packed_attn_fwd(const void* q, const void* k, const void* v, in
 
 // floats of `part` (0: none)
 MX_EXPORT int64_t mx_packed_attn_bwd_floats(int T, int Hq, int Hkv, int D) {
-  if (T <= 0 || Hq <= 0 || Hkv <= 0 || (D != 64 && D != 128)) return 0;
+  if (bad_shape(T, Hq, Hkv, D)) return 0;
+  if (const int n = key_shares(T, Hq, Hkv, D)) return (int64_t)n * 2 * 2 * KB2 * D;
   const int n = key_splits(T, Hq, Hkv, D);
   return n > 1 ? (int64_t)n * 2 * T * Hkv * D : 0;
 }
@@ -1152,8 +1303,10 @@ MX_EXPORT int mx_packed_attn_bwd(const void* q, const void* k, const void* v, in
   a.scale = scale;
   a.fill = fill;
   a.nsplit = key_splits(T, Hq, Hkv, D);
+  a.nshare = key_shares(T, Hq, Hkv, D);
+  a.before = reinterpret_cast<const int64_t*>(order + order_base(T));
   a.part = part;
-  if (a.nsplit > 1 && (!part || ((uintptr_t)part & 15) || part_floats < mx_packed_attn_bwd_floats(T, Hq, Hkv, D)))
+  if (const int64_t n = mx_packed_attn_bwd_floats(T, Hq, Hkv, D); n && (!part || ((uintptr_t)part & 15) || part_floats < n))
     return hipErrorInvalidValue;
   const unsigned nb = (unsigned)((T + 127) / 128);
   if (D == 64) {
@@ -1162,9 +1315,14 @@ MX_EXPORT int mx_packed_attn_bwd(const void* q, const void* k, const void* v, in
     hipLaunchKernelGGL((packed_kmajor_kernel<64>), dim3(nb * Hkv * a.nsplit), dim3(256), 0, s, a);
   } else {
     hipLaunchKernelGGL((packed_qmajor_kernel<128, true>), dim3(nb * Hq), dim3(256), 0, s, a);
-    const unsigned nk = (unsigned)((T + KB2 - 1) / KB2);
     a.order = order + 2 * nb;
-    hipLaunchKernelGGL((packed_kmajor2_kernel<128>), dim3(nk * Hkv * a.nsplit), dim3(256), 0, s, a);
+    const unsigned nk = (unsigned)((T + KB2 - 1) / KB2);
+    if (a.nshare) {
+      hipLaunchKernelGGL((packed_kmajor2_kernel<128, true>), dim3(a.nshare), dim3(256), 0, s, a);
+      hipLaunchKernelGGL(packed_join2_kernel, dim3((a.nshare - 1) * JOIN), dim3(256), 0, s, a);
+      return hipGetLastError();
+    }
+    hipLaunchKernelGGL((packed_kmajor2_kernel<128, false>), dim3(nk * Hkv * a.nsplit), dim3(256), 0, s, a);
   }
   if (a.nsplit > 1) {
     const dim3 grid((unsigned)(((int64_t)T * Hkv * (D / 4) + 255) / 256));

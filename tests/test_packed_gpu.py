@@ -267,3 +267,70 @@ def test_non_finite_values_beside_split_key_blocks(D):
         assert (t[2200:] == 0).all(), name
     within(o[:1290], tuple(x[:1290] for x in want["o"]), "o")
     assert torch.isnan(o[1290:1300]).all() and torch.isnan(grads[1][:1300]).all()
+
+
+@pytest.mark.parametrize("lens,pad,heads", [([1500, 1, 30, 1200, 700], 351, (16, 4)), ([900, 3000], 0, (16, 2)),
+                                            ([1000], 0, (64, 1)), ([5] * 400 + [1800], 7, (24, 8)),
+                                            ([256, 256, 512, 255, 1], 9000, (8, 4))])
+def test_shared_key_heads_over_even_shares(lens, pad, heads):
+    """Grouped heads of 128 with enough work that the key blocks are cut into even shares."""
+    (Hq, Hkv), D = heads, 128
+    T = sum(lens) + pad
+    nv = T - pad
+    assert T * Hq >= 60000
+    q, k, v, do = _inputs(T, Hq, Hkv, D, seed=31)
+    s = ops.pack_sequences(_cu(lens), T, device=DEV)
+    want = attention(q, k, v, lens, Hq, Hkv, D, D ** -0.5, do)
+    q[nv:], k[nv:], v[nv:], do[nv:] = (float("nan"),) * 4
+    o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D)
+    grads = ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D)
+    for name, t in zip(("dq", "dk", "dv"), grads):
+        within(t[:nv], tuple(x[:nv] for x in want[name]), name)
+        assert (t[nv:] == 0).all(), name
+    mine = [torch.full_like(t, 3.0) for t in grads]
+    ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D, dq=mine[0], dk=mine[1], dv=mine[2])
+    for name, a, b in zip(("dq", "dk", "dv"), mine, grads):
+        assert torch.equal(a[:nv], b[:nv]) and (a[nv:] == 3.0).all(), name
+
+
+def test_non_finite_values_beside_even_shares():
+    lens, Hq, Hkv, D = [1900, 2300], 16, 4, 128
+    T = sum(lens) + 10
+    q, k, v, do = _inputs(T, Hq, Hkv, D, seed=32)
+    s = ops.pack_sequences(_cu(lens), T, device=DEV)
+    want = attention(q, k, v, lens, Hq, Hkv, D, D ** -0.5, do)
+    for t in (q, k, v, do):
+        t[1890:1900] = float("nan")
+    o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D)
+    grads = ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D)
+    for name, t in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+        within(t[1900:4200], tuple(x[1900:4200] for x in want[name]), name)
+    within(o[:1890], tuple(x[:1890] for x in want["o"]), "o")
+    assert torch.isnan(grads[1][:1900]).all()
+
+
+def test_shares_of_an_empty_and_a_changed_batch_in_a_graph():
+    Hq, Hkv, D, T = 16, 4, 128, 3900
+    cu = torch.zeros(4, dtype=torch.int64, device=DEV)
+    q, k, v, do = _inputs(T, Hq, Hkv, D, seed=33)
+
+    def go():
+        s = ops.pack_sequences(cu, T)
+        o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D)
+        return (o, *ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D))
+    cu.copy_(_cu([3000, 0, 900]))
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        go()
+    torch.cuda.current_stream().wait_stream(st)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = go()
+    for lens in ([0, 0, 0], [3900, 0, 0], [17, 2000, 1], [3000, 0, 900]):
+        cu.copy_(_cu(lens))
+        g.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in outs]
+        for x, y in zip(got, go()):
+            assert torch.equal(x, y)
