@@ -36,6 +36,11 @@ struct GArgs {
   int tiles_m, tiles_n, gm;
   int act, accumulate;
   int splits, nks;       // EPI 4: K-steps per split
+  // EPI 5: the second product (its K and accumulate are the first's)
+  const uint16_t *a2, *b2;
+  uint16_t* c2;
+  int lda2, ldb2, ldc2, M2, N2, tiles_m2, tiles_n2;
+  int wgs1;              // workgroups of the first
 };
 
 __device__ __forceinline__ float act_fwd(int act, float x) {
@@ -99,9 +104,11 @@ __device__ __forceinline__ i32x4_t tile_rsrc(const uint16_t* base, int rows, int
 
 // EPI 0: C (+)= acc   1: C = acc + bias   2: gate (two column halves)   3: gate gradient
 //     4: fp32 partial of one K range into part[split][M][N] (joined by gated_join_kernel)
-template <bool AKC, bool BKC, int WM, int WN, int FM, int FN, int BKT, int NSLOT, int MINB, int EPI>
+//     5: 0 of two products in one launch, whose rounds of workgroups would each end half empty
+template <bool AKC, bool BKC, int WM, int WN, int FM, int FN, int BKT, int NSLOT, int MINB, int KIND>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(MINB, MINB))) void gated_gemm_kernel(
-    const GArgs g) {
+    const GArgs g0) {
+  constexpr int EPI = KIND == 5 ? 0 : KIND;
   using Gm = Geo<AKC, BKC, WM, WN, FM, FN, BKT, NSLOT>;
   constexpr int BM = Gm::BM, BN = Gm::BN, RA = Gm::RA, RB = Gm::RB, IA = Gm::IA;
   constexpr int PA = Gm::PA, PB = Gm::PB, SLOT = Gm::SLOT, PER = PA + PB;
@@ -114,7 +121,16 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(MI
   const int wm = wave / WN, wn = wave % WN;
   // XCD-contiguous order over groups of gm row tiles
   // (the splits of a tile are adjacent ids)
-  const int wgs = xcd_remap(blockIdx.x, gridDim.x);
+  int wgs = xcd_remap(blockIdx.x, gridDim.x);
+  GArgs g = g0;
+  if constexpr (KIND == 5)
+    if (wgs >= g0.wgs1) {
+      wgs -= g0.wgs1;
+      g.a = g0.a2; g.b = g0.b2; g.c = g0.c2;
+      g.lda = g0.lda2; g.ldb = g0.ldb2; g.ldc = g0.ldc2;
+      g.M = g0.M2; g.N = g0.N2;
+      g.tiles_m = g0.tiles_m2; g.tiles_n = g0.tiles_n2;
+    }
   const int split = EPI == 4 ? wgs % g.splits : 0, wg = EPI == 4 ? wgs / g.splits : wgs;
   const int per = g.gm * g.tiles_n, grp = wg / per, rem = wg - grp * per;
   const int gmr = min(g.gm, g.tiles_m - grp * g.gm);   // (the last group may be smaller)
@@ -551,7 +567,13 @@ int launch(GArgs g, hipStream_t s) {
   const int nk = (g.K + BKT - 1) / BKT;
   g.nks = (nk + g.splits - 1) / g.splits;
   g.splits = (nk + g.nks - 1) / g.nks;              // (no empty split)
-  const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+  int64_t grid = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+  if (EPI == 5) {
+    g.wgs1 = (int)min(grid, (int64_t)INT32_MAX);
+    g.tiles_m2 = (g.M2 + Gm::BM - 1) / Gm::BM;
+    g.tiles_n2 = (g.N2 + Gm::BN - 1) / Gm::BN;
+    grid += (int64_t)g.tiles_m2 * g.tiles_n2;
+  }
   if (grid >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((gated_gemm_kernel<AKC, BKC, WM, WN, FM, FN, BKT, NSLOT, 2, EPI>), dim3((unsigned)grid),
                      dim3(Gm::NT), 0, s, g);
@@ -681,4 +703,22 @@ MX_EXPORT int mx_gated_dw(const void* a, int lda, const void* b, int ldb, void* 
   g.lda = lda; g.ldb = ldb; g.ldc = ldc; g.part = part;
   g.M = M; g.N = N; g.K = T; g.accumulate = accumulate;
   return run<false, false, 0>(tile, splits, g, s);
+}
+
+// two such products over the same T rows in one launch
+MX_EXPORT int mx_gated_dw_pair(const void* a1, int lda1, const void* b1, int ldb1, void* dw1, int ldc1, int M1, int N1,
+                               const void* a2, int lda2, const void* b2, int ldb2, void* dw2, int ldc2, int M2, int N2,
+                               int T, int accumulate, int tile, hipStream_t s) {
+  if (T <= 0 || bad_dim(M1) || bad_dim(N1) || bad_rows(a1, lda1, M1) || bad_rows(b1, ldb1, N1) ||
+      bad_rows(dw1, ldc1, N1) || bad_dim(M2) || bad_dim(N2) || bad_rows(a2, lda2, M2) || bad_rows(b2, ldb2, N2) ||
+      bad_rows(dw2, ldc2, N2))
+    return hipErrorInvalidValue;
+  GArgs g{};
+  g.a = (const uint16_t*)a1; g.b = (const uint16_t*)b1; g.c = (uint16_t*)dw1;
+  g.lda = lda1; g.ldb = ldb1; g.ldc = ldc1;
+  g.M = M1; g.N = N1; g.K = T; g.accumulate = accumulate;
+  g.a2 = (const uint16_t*)a2; g.b2 = (const uint16_t*)b2; g.c2 = (uint16_t*)dw2;
+  g.lda2 = lda2; g.ldb2 = ldb2; g.ldc2 = ldc2; g.M2 = M2; g.N2 = N2;
+  g.splits = 1;
+  return run_tile<false, false, 5>(tile, g, s);
 }

@@ -130,6 +130,7 @@ SIGNATURES = {
     "mx_gated_dgate": [P, I, P, I, P, P, P, I, I, I, I, I, P],
     "mx_gated_dx": [P, P, I, P, I, I, I, I, I, P, P],
     "mx_gated_dw": [P, I, P, I, P, I, I, I, I, I, I, I, P, P],
+    "mx_gated_dw_pair": [P, I, P, I, P, I, I, I, P, I, P, I, P, I, I, I, I, I, I, P],
     # rope.hip
     "mx_rope": [P, I64, I, I, I, I, I, I, I, P, P, P, I, P],
     # vision.hip

@@ -116,8 +116,21 @@ _TILES = ((128, 128, 2, 1.14, 5.0), (256, 256, 1, 1.69, 8.0), (256, 256, 1, 1.72
 _PLANS = {}
 
 
+def _estimate(tile, wgs, steps):
+    """us of ``wgs`` workgroups of ``steps`` 64-deep steps each."""
+    _, _, per, step, fix = _TILES[tile]
+    if per == 2 and wgs <= 256:      # alone on its CU: the two-slot ring waits for memory
+        step = 0.97
+    return -(-wgs // (256 * per)) * (steps * step + fix)
+
+
+def _count(tile, M, N):
+    bm, bn = _TILES[tile][:2]
+    return -(-M // bm) * -(-N // bn)
+
+
 def _plan(kind, M, N, K):
-    """(tile, splits) of one product, M x N over K (N: columns of both halves for "gate"): the
+    """(tile, splits, us) of one product, M x N over K (N: columns of both halves for "gate"): the
     least estimated time.  Big tiles move the fewest operand bytes per product, so they win where
     they fill whole rounds (4096 x 4096 x 10880 "down": 287 us with 256 x 256 tiles, 387 with 128 x
     128); few tiles leave CUs idle, so smaller ones with a deeper ring win (1003 x 768 x 2048 "gate":
@@ -126,25 +139,40 @@ def _plan(kind, M, N, K):
     key = (kind, M, N, K)
     best = _PLANS.get(key)
     if best is None:
-        steps, cost = -(-K // 64), None
-        for tile, (bm, bn, per, step, fix) in enumerate(_TILES):
-            tiles = -(-M // bm) * -(-N // bn)
+        steps = -(-K // 64)
+        for tile in range(len(_TILES)):
+            tiles = _count(tile, M, N)
             for splits in ((1, 2, 4, 8) if kind in ("down", "dx", "dw") else (1,)):
                 if splits > 1 and (tiles * splits > 256 or steps < 8 * splits):
                     break
-                wgs = tiles * splits
-                rounds = -(-wgs // (256 * per))
-                if per == 2 and wgs <= 256:      # alone on its CU: the two-slot ring waits for memory
-                    step = 0.97
-                est = rounds * (-(-steps // splits) * step + fix)
+                est = _estimate(tile, tiles * splits, -(-steps // splits))
                 if splits > 1:                   # partials written and read, one more launch
                     est += 4.0 + splits * M * N * 8 / 4e6
-                if cost is None or est < cost:
-                    cost, best = est, (tile, splits)
-        if len(_PLANS) > 4096:
-            _PLANS.clear()
-        _PLANS[key] = best
+                if best is None or est < best[2]:
+                    best = (tile, splits, est)
+        _keep(key, best)
     return best
+
+
+def _plan_pair(T, H, F, Ho):
+    """The tile of both weight gradients in one launch, or None where two are faster: together they
+    leave one round of workgroups unfilled, not two (4096 x 1024 x 2688: 64 us, apart 58 + 40; 4096 x
+    4096 x 10880: 911 and 630 + 321; 2048 x 2048 x 5504 fills its rounds: 154 and 97 + 56)."""
+    key = ("pair", T, H, F, Ho)
+    if key not in _PLANS:
+        best, cost = None, _plan("dw", 2 * F, H, T)[2] + _plan("dw", Ho, F, T)[2] + 2.0
+        for tile in range(len(_TILES)):
+            est = _estimate(tile, _count(tile, 2 * F, H) + _count(tile, Ho, F), -(-T // 64))
+            if est < cost:
+                best, cost = tile, est
+        _keep(key, best)
+    return _PLANS[key]
+
+
+def _keep(key, plan):
+    if len(_PLANS) > 4096:
+        _PLANS.clear()
+    _PLANS[key] = plan
 
 
 def _split_ws(splits, M, N, device):
@@ -177,7 +205,7 @@ def gated_mlp_fwd(x, w1, b1, w2, b2, act: str = "silu", save: bool = True):
         s = _lib.stream()
         _lib.call("mx_gated_fwd", x_, ldx, w1_, ld1, b1_, _lib.ptr(pre), h.data_ptr(), T, H, F, ACTS[act],
                   _plan("gate", T, 2 * F, H)[0], s)
-        tile, splits = _plan("down", T, Ho, F)
+        tile, splits, _ = _plan("down", T, Ho, F)
         part = _split_ws(splits, T, Ho, x.device)
         _lib.call("mx_gated_down", h.data_ptr(), w2_, ld2, b2_, y.data_ptr(), T, Ho, F, tile, splits, _lib.ptr(part),
                   s)
@@ -234,7 +262,7 @@ def gated_mlp_bwd(dy, x, pre, h, w1, b1, w2, b2, act: str = "silu", dw1=None, db
         s = _lib.stream()
         dpre = torch.empty(T, 2 * F, dtype=x.dtype, device=x.device)
         part = buf = None
-        tile, _ = _plan("dgate", T, F, Ho)
+        tile = _plan("dgate", T, F, Ho)[0]
         bm = _lib.query("mx_gated_tile", tile, 0)
         nparts = (T + bm - 1) // bm * _lib.query("mx_gated_tile", tile, 2)
         if db1 is not None:
@@ -244,14 +272,19 @@ def gated_mlp_bwd(dy, x, pre, h, w1, b1, w2, b2, act: str = "silu", dw1=None, db
         dx = None
         if need_dx:
             dx = torch.empty(T, H, dtype=x.dtype, device=x.device)
-            tile, splits = _plan("dx", T, H, 2 * F)
+            tile, splits, _ = _plan("dx", T, H, 2 * F)
             ws = _split_ws(splits, T, H, x.device)
             _lib.call("mx_gated_dx", _lib.ptr(dpre), _lib.ptr(w1), _ld(w1), _lib.ptr(dx), T, H, 2 * F, tile, splits,
                       _lib.ptr(ws), s)
         if need_dw:
-            for a, b, out in ((dpre, x, dw1), (dy, h, dw2)):
+            pair = _plan_pair(T, H, F, Ho)
+            if pair is not None:
+                _lib.call("mx_gated_dw_pair", _lib.ptr(dpre), 2 * F, _lib.ptr(x), _ld(x), _lib.ptr(dw1), _ld(dw1),
+                          2 * F, H, _lib.ptr(dy), _ld(dy), _lib.ptr(h), F, _lib.ptr(dw2), _ld(dw2), Ho, F, T,
+                          int(accumulate), pair, s)
+            for a, b, out in ((dpre, x, dw1), (dy, h, dw2)) if pair is None else ():
                 (m, n) = out.shape
-                tile, splits = _plan("dw", m, n, T)
+                tile, splits, _ = _plan("dw", m, n, T)
                 ws = _split_ws(splits, m, n, x.device)
                 _lib.call("mx_gated_dw", _lib.ptr(a), _ld(a), _lib.ptr(b), _ld(b), _lib.ptr(out), _ld(out), T, m, n,
                           int(accumulate), tile, splits, _lib.ptr(ws), s)

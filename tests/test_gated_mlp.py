@@ -279,3 +279,29 @@ def test_gpu_captured_and_replayed():
         torch.cuda.synchronize()
         for a, b in zip([t.clone() for t in outs], go()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("tile", range(5))
+@pytest.mark.parametrize("T,H,F,Ho", [(65, 8, 40, 264), (200, 264, 136, 72), (1003, 768, 520, 768)])
+def test_paired_weight_gradients_equal_single_ones(monkeypatch, T, H, F, Ho, tile, accumulate):
+    """Both weight gradients in one launch: the bits of two launches with the same tile."""
+    import mxtrain.ops.gated as gated
+    gen = torch.Generator().manual_seed(T + tile)
+    r = lambda *s: torch.randn(*s, generator=gen).to(torch.bfloat16).cuda()
+    x, w1, w2, dy = r(T, H), r(2 * F, H), r(Ho, F), r(T, Ho)
+    pre, h = r(T, 2 * F), r(T, F)
+    start = r(2 * F, H), r(Ho, F)
+    monkeypatch.setattr(gated, "_plan", lambda *a: (tile, 1, 0.0))
+
+    def go(pair):
+        monkeypatch.setattr(gated, "_plan_pair", lambda *a: pair)
+        wide = torch.full((2 * F, H + 16), 3.0, dtype=torch.bfloat16, device="cuda")
+        wide[:, :H] = start[0]
+        dw1, dw2 = wide[:, :H], start[1].clone()
+        gated.gated_mlp_bwd(dy, x, pre, h, w1, None, w2, None, dw1=dw1, dw2=dw2, accumulate=accumulate)
+        assert (wide[:, H:] == 3.0).all()
+        return dw1, dw2
+    for a, b in zip(go(tile), go(None)):
+        assert torch.equal(a, b)
