@@ -158,48 +158,38 @@ __global__ __launch_bounds__(SORT_NT) void sort_scatter_kernel(const SortArgs a)
   }
 }
 
-// The whole sort of up to SMALL tokens in one workgroup and one launch, the pairs in LDS: at 4096
-// tokens two digit passes cost less than the launches of the block form (17 us).
+// Few tokens: the place of a token is the number of keys below its own, and of equal ones before it, so
+// one launch counts it -- T^2 compares of keys in LDS, little at T tokens against the latency of radix
+// passes (6.0 us at 4096 tokens, where a radix sort in one workgroup took 13.3 and the block form 17;
+// the whole gradient of 8192 tokens, 50304 rows of 64: 28 us, and 38 by the block form, which takes no
+// more at 16384, where this would take four times as many compares).  A workgroup places 16
+// tokens: lane (q, i) of wave w compares token i with every 64th group of four keys.
 constexpr int SMALL = 8192;
-__global__ __launch_bounds__(SORT_NT) void sort_small_kernel(const SortArgs a, int passes) {
-  __shared__ int keys[2][SMALL];
-  __shared__ uint16_t idx[2][SMALL];
-  __shared__ int wcnt[SORT_NW << MAX_BITS];
-  __shared__ int wsum[SORT_NW];
-  const int R = 1 << a.bits, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, T = a.T;
-  const int share = ((T + 64 * SORT_NW - 1) / (64 * SORT_NW)) * 64;
-  const int s0 = min(T, w * share), s1 = min(T, s0 + share);
-  for (int t = tid; t < T; t += SORT_NT) {
-    keys[0][t] = sort_key(a, t);
-    idx[0][t] = (uint16_t)t;
+__global__ __launch_bounds__(SORT_NT) void sort_small_kernel(const SortArgs a) {
+  __shared__ __attribute__((aligned(16))) int keys[SMALL];
+  __shared__ int cnt[SORT_NW][16];
+  const int T = a.T, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int T4 = (T + 3) & ~3;
+  for (int t = tid; t < T4; t += SORT_NT) keys[t] = t < T ? sort_key(a, t) : INT32_MAX;   // (above every key)
+  __syncthreads();
+  const int i = min((int)blockIdx.x * 16 + (lane & 15), T - 1), mine = keys[i];
+  int n = 0;
+#pragma unroll 4
+  for (int u = w * 4 + (lane >> 4); u < T4 / 4; u += SORT_NW * 4) {
+    const int4 k = *reinterpret_cast<const int4*>(keys + 4 * u);
+    const int below = mine + (4 * u + 3 < i ? 1 : 0);
+    n += (int)(k.x < below) + (int)(k.y < below) + (int)(k.z < below) + (int)(k.w < below);
   }
-  for (int p = 0; p < passes; ++p) {
-    const int shift = p * a.bits, in = p & 1, out = in ^ 1;
-    for (int i = tid; i < SORT_NW * R; i += SORT_NT) wcnt[i] = 0;
-    __syncthreads();
-    for (int t = s0 + lane; t < s1; t += 64) atomicAdd(&wcnt[w * R + ((keys[in][t] >> shift) & (R - 1))], 1);
-    __syncthreads();
-    int total = 0;
-    if (tid < R)
-      for (int i = 0; i < SORT_NW; ++i) total += wcnt[i * R + tid];
-    digit_slots(wcnt, wsum, R, total, 0);
-    for (int c0 = s0; c0 < s1; c0 += 64) {
-      const int t = c0 + lane;
-      const bool live = t < s1;
-      const int key = live ? keys[in][t] : 0;
-      const int slot = take_slot(wcnt + w * R, (key >> shift) & (R - 1), a.bits, live, lane);
-      if (live) {
-        keys[out][slot] = key;
-        idx[out][slot] = idx[in][t];
-      }
-    }
-    __syncthreads();
-  }
-  const int fin = passes & 1;
-  for (int t = tid; t < T; t += SORT_NT) {
-    a.kout[t] = keys[fin][t];
-    a.iout[t] = idx[fin][t];
-  }
+  n += __shfl_xor(n, 16);
+  n += __shfl_xor(n, 32);
+  if (lane < 16) cnt[w][lane] = n;
+  __syncthreads();
+  if (tid >= 16 || (int)blockIdx.x * 16 + tid >= T) return;
+  int place = 0;
+  for (int x = 0; x < SORT_NW; ++x) place += cnt[x][tid];
+  for (int t = i & ~3; t < i; ++t) place += keys[t] == mine;     // equal ones of its own four
+  a.kout[place] = mine;
+  a.iout[place] = i;
 }
 
 // ------------------------------------------------------------------------------ sums
@@ -380,7 +370,7 @@ MX_EXPORT int mx_embedding_bwd(const void* ids, int64_t vstart, const void* dout
   float* part = (float*)(hist + (((int64_t)p.blocks << p.bits) + 3 & ~3ll));
   SortArgs a{(const int64_t*)ids, vstart, V, T, p.tpb, nullptr, nullptr, k0, i0, hist, 0, p.bits};
   if (T <= SMALL) {
-    hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(SORT_NT), 0, s, a, p.passes);
+    hipLaunchKernelGGL(sort_small_kernel, dim3((T + 15) / 16), dim3(SORT_NT), 0, s, a);
     a.kin = k0;
     a.iin = i0;
   }
