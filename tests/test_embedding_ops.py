@@ -205,3 +205,18 @@ def test_gpu_captured_and_replayed():
         torch.cuda.synchronize()
         for x, y in zip([t.clone() for t in outs], go()):
             assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["any", "one", "range", "outside"])
+@pytest.mark.parametrize("T", [4095, 8191, 8192, 8193])
+def test_gpu_both_ways_to_sort_keep_token_order(T, kind):
+    """Around the most tokens that are placed by counting; the sums are those of token order."""
+    gen = torch.Generator().manual_seed(T)
+    V, H = 900, 16
+    ids = _ids(kind, T, V, gen).to("cuda")
+    dout = torch.randn(T, H, generator=gen).to(torch.bfloat16).to("cuda")
+    val, bound = _oracle_bwd(ids, dout, V, 0.75)
+    first = ops.embedding_bwd(ids, dout, V, 0.75)
+    _within(first, val, bound)
+    assert torch.equal(first, ops.embedding_bwd(ids, dout, V, 0.75))
