@@ -10,7 +10,7 @@
 // takes the keys [start(first row), last row], so a block may hold the end of one sequence and
 // the beginning of others and many short sequences cost no padding; a 32 x 32 subtile is skipped,
 // taken whole, or masked per element (start(i) <= j <= i is one unsigned compare).  Rows behind
-// the last sequence (a batch padded to a fixed size) are never read.
+// the last sequence (a batch padded to a fixed size) never matter, whatever they hold.
 //
 // A masked score has p = 0, but 0 * NaN = NaN inside a matrix product: a masked subtile whose
 // V (dQ: K; dK / dV: Q, dO) rows hold a non-finite value marks its wave, and the wave's rows are
@@ -23,7 +23,6 @@
 
 using namespace mx;
 using namespace mx::flash;
-using mx::gemm::buffer_rsrc;
 using mx::gemm::i32x4_t;
 
 namespace {

@@ -260,6 +260,18 @@ def on_device(t):
     return _SAME_DEVICE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
+def overlap(T, a, b) -> bool:
+    """Whether two [T, width] bf16 matrices, each (address, row stride, width), share memory (column ranges
+    of one buffer do not)."""
+    if b[0] < a[0]:
+        a, b = b, a
+    (pa, lda, wa), (pb, ldb, wb) = a, b
+    if pb >= pa + 2 * ((T - 1) * lda + wa):
+        return False
+    c = (pb - pa) % (2 * lda)
+    return lda != ldb or c < 2 * wa or c + 2 * wb > 2 * lda
+
+
 def rows_of(t, rows, cols, dev, ld_max):
     """(address, row stride) of a bfloat16 [rows, cols] matrix on device index ``dev`` that the
     kernels take in place -- unit column stride, 16-byte aligned rows that do not overlap -- or

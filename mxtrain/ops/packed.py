@@ -7,8 +7,11 @@ batch, shared by every layer and by forward and backward.  Tensors are token-maj
 ``ops/attention.py``; ``lse`` is the base-2 log-sum-exp [Hq, T] the backward needs.
 
 Rows behind the last sequence (a batch padded to a fixed size, so a captured step keeps its
-shapes) are never read: in tensors the op allocates they are zero, in buffers the caller passes
-they are left as they were.
+shapes) never matter, whatever they hold: in tensors the op allocates they are zero, in buffers the
+caller passes they are left as they were.
+
+On the GPU scores, softmax statistics and sums are fp32; P and dS are rounded once to bf16 as operands of
+the matrix products, and delta = do . o is taken from the bf16 ``o`` that forward returned.
 """
 from __future__ import annotations
 
@@ -178,6 +181,13 @@ def _emit(val, buf, seqs):
     return buf
 
 
+def _apart(name, T, outs, ins):
+    """Results that lie over an operand, or over each other, would be read after they are written."""
+    for i, a in enumerate(outs):
+        if any(_lib.overlap(T, a, b) for b in ins + outs[:i]):
+            raise ValueError(f"{name}: results must not lie over the operands or over each other")
+
+
 # ------------------------------------------------------------------ forward / backward
 def packed_attn_fwd(q, k, v, seqs: PackedSequences, Hq: int, Hkv: int, D: int, scale: Optional[float] = None,
                     out=None):
@@ -192,6 +202,8 @@ def packed_attn_fwd(q, k, v, seqs: PackedSequences, Hq: int, Hkv: int, D: int, s
         raise ValueError("packed_attn_fwd: unsupported arguments")
     T = seqs.total
     (q_, ldq), (k_, ldk), (v_, ldv), o_ = m
+    if out is not None:
+        _apart("packed_attn_fwd", T, [(*o_, Hq * D)], [(q_, ldq, Hq * D), (k_, ldk, Hkv * D), (v_, ldv, Hkv * D)])
     with _lib.on_device(q):
         o = out if out is not None else torch.empty(T, Hq * D, dtype=q.dtype, device=q.device)
         lse = torch.empty(Hq, T, dtype=torch.float32, device=q.device)
@@ -226,8 +238,10 @@ def packed_attn_bwd(dout, q, k, v, o, lse, seqs: PackedSequences, Hq: int, Hkv: 
     if (dk is not None) != given or (dv is not None) != given:
         raise ValueError("packed_attn_bwd: give all of dq, dk, dv or none")
     (q_, ldq), (k_, ldk), (v_, ldv), (o_, ldo), (do_, lddo), *grads = m
-    if given and {g[0] for g in grads} & {q_, k_, v_, o_, do_}:
-        raise ValueError("packed_attn_bwd: dq, dk, dv must not lie over q, k, v, o or dout (read after they are written)")
+    if given:
+        wide, narrow = Hq * D, Hkv * D
+        _apart("packed_attn_bwd", T, [(*g, w) for g, w in zip(grads, (wide, narrow, narrow))],
+               [(q_, ldq, wide), (k_, ldk, narrow), (v_, ldv, narrow), (o_, ldo, wide), (do_, lddo, wide)])
     with _lib.on_device(q):
         if not given:
             dq = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device)

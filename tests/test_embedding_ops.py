@@ -220,3 +220,11 @@ def test_gpu_both_ways_to_sort_keep_token_order(T, kind):
     first = ops.embedding_bwd(ids, dout, V, 0.75)
     _within(first, val, bound)
     assert torch.equal(first, ops.embedding_bwd(ids, dout, V, 0.75))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_gradient_over_its_input_is_refused(device):
+    ids = torch.tensor([0, 1, 0, 3], device=device)
+    d = torch.ones(4, 8, dtype=torch.bfloat16, device=device)
+    with pytest.raises(ValueError):
+        ops.embedding_bwd(ids, d, 4, out=d)

@@ -305,3 +305,15 @@ def test_paired_weight_gradients_equal_single_ones(monkeypatch, T, H, F, Ho, til
         return dw1, dw2
     for a, b in zip(go(tile), go(None)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_gradient_buffers_over_operands_are_refused(device):
+    T, H, F = 16, 8, 8
+    x, w1, b1, w2, b2, dy = _make(T, H, F, 16, True, device=device)
+    y, pre, h = ops.gated_mlp_fwd(x, w1, b1, w2, b2)
+    for grads in ({"dw1": x}, {"dw2": dy}, {"dw1": h}, {"db1": torch.empty_like(b1)} | {"db2": None}):
+        if "db1" in grads:
+            grads = {"db1": grads["db1"], "db2": grads["db1"]}       # (2 F = Ho)
+        with pytest.raises(ValueError):
+            ops.gated_mlp_bwd(dy, x, pre, h, w1, b1, w2, b2, **grads)

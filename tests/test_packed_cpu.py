@@ -83,3 +83,25 @@ def test_buffers_keep_the_rows_behind():
     out = torch.full((8, 16), 7.0)
     ops.packed_attn_fwd(q, q, q, s, 1, 1, 16, out=out)
     assert (out[5:] == 7.0).all() and not (out[:5] == 7.0).any()
+
+
+def test_overlap_of_strided_matrices():
+    from mxtrain.ops import _lib
+    buf = torch.zeros(10, 96, dtype=torch.bfloat16)
+    m = lambda t: (t.data_ptr(), t.stride(0), t.shape[1])
+    owned = torch.zeros(40, 32, dtype=torch.int64)      # a plain count of who touches what
+
+    def touch(t):
+        owned.zero_()
+        own = owned.view(-1)[:960].view(10, 96)
+        r0, c0 = divmod((t.data_ptr() - buf.data_ptr()) // 2, 96)
+        own[r0:r0 + t.shape[0], c0:c0 + t.shape[1]] = 1
+        return own.clone()
+    views = [buf[a:a + 6, c:c + w] for a in (0, 3, 4) for c, w in ((0, 32), (32, 32), (64, 32), (16, 40), (0, 96))]
+    for x in views:
+        for y in views:
+            assert _lib.overlap(6, m(x), m(y)) >= bool((touch(x) & touch(y)).any())
+    a, b = buf[:, :32], buf[:, 32:]
+    assert not _lib.overlap(10, m(a), m(b)) and not _lib.overlap(10, m(b), m(a))
+    assert _lib.overlap(10, m(a), m(a)) and _lib.overlap(10, m(a), (a.data_ptr() + 64, 200, 8))
+    assert not _lib.overlap(10, m(buf), m(torch.zeros(10, 96, dtype=torch.bfloat16)))

@@ -334,3 +334,21 @@ def test_shares_of_an_empty_and_a_changed_batch_in_a_graph():
         got = [t.clone() for t in outs]
         for x, y in zip(got, go()):
             assert torch.equal(x, y)
+
+
+def test_results_over_operands_are_refused():
+    T, H, D = 40, 2, 64
+    s = ops.pack_sequences(_cu([T]), T, device=DEV)
+    buf = torch.randn(T, 8 * H * D, device=DEV).to(torch.bfloat16)
+    q, k, v, do, a, b, c, e = buf.split(H * D, 1)
+    o, lse = ops.packed_attn_fwd(q, k, v, s, H, H, D, out=a)       # other columns of the operands' buffer
+    for bad in (q, k, v, buf[:, 64:64 + H * D]):
+        with pytest.raises(ValueError):
+            ops.packed_attn_fwd(q, k, v, s, H, H, D, out=bad)
+    want = ops.packed_attn_bwd(do, q, k, v, o, lse, s, H, H, D)
+    got = ops.packed_attn_bwd(do, q, k, v, o, lse, s, H, H, D, dq=b, dk=c, dv=e)
+    for x, y in zip(want, got):
+        assert torch.equal(x, y)
+    for bad in ((b, c, c), (b, b, c), (o, b, c), (b, c, do), (b, k, c)):
+        with pytest.raises(ValueError):
+            ops.packed_attn_bwd(do, q, k, v, o, lse, s, H, H, D, dq=bad[0], dk=bad[1], dv=bad[2])
