@@ -14,6 +14,10 @@
 // what lies past a tile's rows reads zero, so any number of tokens and any feature count that is a
 // multiple of 8 is taken without padding.  16 x 16 x 32 MFMA with the weight (column) operand
 // first, so that a lane holds 4 consecutive columns of a row.
+//
+// Large products are bound by their K loop: at 128 x 64 a wave the fragment reads from LDS take as long
+// as the matrix pipe (1.1 - 1.25 PFLOP/s; forward and backward of 4096 x 4096 x 10880 in 2.95 ms).  Short
+// ones (4096 x 1024 x 2688: 0.27 ms) by rounds of workgroups that fill and drain for 16 - 84 steps.
 #include "gemm_common.h"
 
 #include <type_traits>
@@ -425,7 +429,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(MI
 // A workgroup takes 16 output columns (of both halves for the gate) and its NW waves split K, so
 // that even a 1024-column product has hundreds of waves with all their loads in flight; no LDS on
 // the way in (a weight is used once), partial sums meet in LDS.  Lane (G, i) loads row i, k 8G ..
-// 8G + 7 of a 16 x 32 block; NG groups of 16 tokens.
+// 8G + 7 of a 16 x 32 block; NG groups of 16 tokens.  Bound by memory latency: 1024 x 2688, one token,
+// 16.5 MB of weights in 5.1 (gate) + 4.3 us, 1.8 TB/s.
 template <int NG, bool DUAL, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void gated_few_kernel(const GArgs g) {
   constexpr int NH = DUAL ? 2 : 1;
@@ -516,7 +521,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
   *reinterpret_cast<uint2*>(g.c + (size_t)m * g.ldc + col) =
       make_uint2(pack2(v[0][0], v[0][1]), pack2(v[0][2], v[0][3]));
 }
-constexpr int kFewTokens = 64;
+// Up to 16 tokens always; up to 64 while the products are small, for every further group of 16 reads x and
+// multiplies again beside the one read of the weights, where a tile of 128 rows does so for nothing (block
+// without `pre`, few-token form and tiles, us: 1 token 1024 x 2688 9.4 and 23, 64 tokens 22.5 and 24.5;
+// 2048 x 5504: 16 tokens 28 and 34, 32 tokens 36 and 35, 64 tokens 53 and 36; 4096 x 10880: 1 token 50 and
+// 62, 16 tokens 62 and 62, 64 tokens 130 and 65).
+bool few_tokens(const GArgs& g) {
+  return g.M <= 16 || (g.M <= 64 && (int64_t)g.M * g.K * g.N <= 320000000);
+}
 template <bool DUAL>
 int run_few(const GArgs& g, hipStream_t s) {
   const dim3 grid((g.N + 15) / 16);
@@ -648,7 +660,7 @@ MX_EXPORT int mx_gated_fwd(const void* x, int ldx, const void* w1, int ldw, cons
   g.bias = (const uint16_t*)b1;
   g.lda = ldx; g.ldb = ldw; g.ldc = F;
   g.M = M; g.N = F; g.K = K; g.act = act;
-  if (M <= kFewTokens) return run_few<true>(g, s);
+  if (few_tokens(g)) return run_few<true>(g, s);
   return run<true, true, 2>(tile, 1, g, s);
 }
 
@@ -662,7 +674,7 @@ MX_EXPORT int mx_gated_down(const void* h, const void* w2, int ldw, const void* 
   g.a = (const uint16_t*)h; g.b = (const uint16_t*)w2; g.c = (uint16_t*)y; g.bias = (const uint16_t*)b2;
   g.lda = K; g.ldb = ldw; g.ldc = N; g.part = part;
   g.M = M; g.N = N; g.K = K;
-  if (M <= kFewTokens) return run_few<false>(g, s);
+  if (few_tokens(g)) return run_few<false>(g, s);
   return run<true, true, 1>(tile, splits, g, s);
 }
 

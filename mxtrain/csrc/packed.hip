@@ -217,7 +217,10 @@ __device__ __forceinline__ int pair_rank(int rank, int n) {
 // ============================================================================ query-major
 // Forward, and dQ of the backward.  Four waves of 32 query rows; query on the MFMA lane
 // (S^T = K Q^T, O^T = V^T P^T), so the softmax statistics are lane-local plus one half exchange.
-// K / V tiles of BK keys arrive by LDS-DMA into a two-slot ring, one barrier per tile.
+// K / V tiles of BK keys arrive by LDS-DMA into a two-slot ring, one barrier per tile.  Two workgroups a
+// CU, so that one's exponentials run beside the other's products: 16384 tokens in one, 32 heads of 128,
+// forward 2.4 ms (0.92 PFLOP/s), dQ 2.9 (1.13); 4096 of ~300, 16 heads of 64, bound by the latency of a
+// block's few tiles, 20 and 23 us.
 template <int D, bool DQ>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void packed_qmajor_kernel(const PArgs a) {
   constexpr int BQ = 128, BK = D == 64 ? 128 : 64, NSUB = BK / 32, NKK = D / 16, NDT = D / 32;
@@ -836,8 +839,10 @@ packed_kmajor_kernel(const PArgs a) {
 // D = 128.  Two 32-key groups per wave, one wave per SIMD: every Q / dO fragment read from LDS feeds
 // two MFMAs (a 32-key wave needs 1408 LDS cycles per 1024 MFMA cycles of the four SIMDs -- the
 // transposed reads run at half rate --, this one 1408 per 2048), and the accumulators of both groups
-// (256 registers), their K and V rows (128) and S, dP (64) just fit the 512 registers.
-// A workgroup holds 256 keys.
+// (256 registers), their K rows and half of V (96; the rest is read again from LDS) and S, dP (64) fit
+// the 512 registers.  A workgroup holds 256 keys.  16384 tokens in one, 32 heads: 4.1 ms, 1.07 PFLOP/s,
+// the matrix pipe busy 45 % of the time: no other wave runs beside a wave's own vector work.
+//
 // MFMA with its accumulator in ordinary registers.  The compiler gives every MFMA of a kernel that
 // needs accumulation registers an accumulator there; dK and dV of 64 keys take all 256 of them, and
 // it moved S and dP in and out of them at every subtile.  Written as asm, so the wait between the

@@ -317,3 +317,14 @@ def test_gradient_buffers_over_operands_are_refused(device):
             grads = {"db1": grads["db1"], "db2": grads["db1"]}       # (2 F = Ho)
         with pytest.raises(ValueError):
             ops.gated_mlp_bwd(dy, x, pre, h, w1, b1, w2, b2, **grads)
+
+
+@gpu
+@pytest.mark.parametrize("T", [16, 17, 38, 39, 64])
+def test_gpu_few_tokens_of_wide_features(T):
+    """Around the most tokens of the weight-streaming form, where that depends on the product's size."""
+    H, F = 2048, 4096
+    x, w1, b1, w2, b2, _ = _make(T, H, F, H, True, seed=T, device=DEV)
+    y, pre, h = ops.gated_mlp_fwd(x, w1, b1, w2, b2)
+    _within(y, _oracle("silu", x, w1, b1, w2, b2)["y"], "y")
+    assert torch.equal(ops.gated_mlp_fwd(x, w1, b1, w2, b2, save=False)[0], y)
