@@ -606,6 +606,7 @@ constexpr Tile kTiles[] = {
     {256, 256, 2},   // 2: 8 waves of 128 x 64, 32-deep steps, 4 slots
     {128, 128, 4},   // 3: 8 waves of 32 x 64, 64-deep steps, 4 slots
     {256, 128, 4},   // 4: 8 waves of 64 x 64, 64-deep steps, 3 slots
+    {64, 128, 2},    // 5: 4 waves of 32 x 64, 64-deep steps, 3 slots (not for weight gradients)
 };
 constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
 
@@ -617,6 +618,9 @@ int run_tile(int tile, const GArgs& g, hipStream_t s) {
     case 2: return launch<AKC, BKC, 2, 4, 8, 4, 32, 4, EPI>(g, s);
     case 3: return launch<AKC, BKC, 4, 2, 2, 4, 64, 4, EPI>(g, s);
     case 4: return launch<AKC, BKC, 4, 2, 4, 4, 64, 3, EPI>(g, s);
+    case 5:
+      if constexpr (AKC) return launch<AKC, BKC, 2, 2, 2, 4, 64, 3, EPI>(g, s);
+      return hipErrorInvalidValue;
     default: return hipErrorInvalidValue;
   }
 }

@@ -108,20 +108,24 @@ def _mats(act, x, w1, b1, w2, b2):
 
 
 # ------------------------------------------------------------------ tiles
-# Per tile of csrc/gated.hip: (rows, columns, workgroups per CU, us per 64-deep step, us per round of
-# workgroups beside the steps), fitted to one MI355X over 4096 x 4096 x 10880 (steps) and
-# 4096 x 1024 x 2688 (rounds); a round is one workgroup on every slot of the 256 CUs.
-_TILES = ((128, 128, 2, 1.14, 5.0), (256, 256, 1, 1.69, 8.0), (256, 256, 1, 1.72, 5.0), (128, 128, 1, 0.62, 4.0),
-          (256, 128, 1, 0.985, 5.0))
+# Per tile of csrc/gated.hip: rows, columns, workgroups per CU; us per 64-deep step, the same of a
+# workgroup alone on its CU; us per round of workgroups (one on every slot of the 256 CUs) beside the
+# steps, more of it where the epilogue reads and writes as much as the gate gradient's, and once.
+# Fitted to one MI355X over 4096 x 4096 x 10880 (steps), 4096 x 1024 x 2688 (rounds) and, the small
+# tile, 1003 x 768 x 2048 and 300 x 512 x 1376.
+_TILES = ((128, 128, 2, 1.14, 0.97, 5.0, 3.5, 0.0), (256, 256, 1, 1.69, 1.69, 8.0, 33.0, 0.0),
+          (256, 256, 1, 1.72, 1.72, 5.0, 30.0, 0.0), (128, 128, 1, 0.62, 0.62, 4.0, 4.2, 0.0),
+          (256, 128, 1, 0.985, 0.985, 5.0, 7.5, 0.0), (64, 128, 2, 0.57, 0.45, 2.5, 3.6, 6.0))
+_DW_TILES = 5          # (the last one does not take operands whose rows are the contraction)
 _PLANS = {}
 
 
-def _estimate(tile, wgs, steps):
+def _estimate(tile, wgs, steps, kind=""):
     """us of ``wgs`` workgroups of ``steps`` 64-deep steps each."""
-    _, _, per, step, fix = _TILES[tile]
-    if per == 2 and wgs <= 256:      # alone on its CU: the two-slot ring waits for memory
-        step = 0.97
-    return -(-wgs // (256 * per)) * (steps * step + fix)
+    _, _, per, step, alone, fix, more, once = _TILES[tile]
+    if wgs <= 256:
+        step, once = alone, once / 4
+    return -(-wgs // (256 * per)) * (steps * step + fix + (more if kind == "dgate" else 0.0)) + once
 
 
 def _count(tile, M, N):
@@ -135,17 +139,20 @@ def _plan(kind, M, N, K):
     they fill whole rounds (4096 x 4096 x 10880 "down": 287 us with 256 x 256 tiles, 387 with 128 x
     128); few tiles leave CUs idle, so smaller ones with a deeper ring win (1003 x 768 x 2048 "gate":
     12.6 us against 24.9), and a long K is split once the tiles cover less than half of the chip
-    (its "dx": 21.2 us in 4 splits, 40 us in one)."""
+    (its "dx": 21.2 us in 4 splits, 40 us in one).  Tiles of 64 rows, two workgroups a CU, run one's
+    epilogue beside the other's loop, which the gate gradient gains from most (4096 x 1024 x 2688: 50
+    us, 54 with 128 x 128, 61 with 256 x 256; 700 x 2048 x 5504: 31 and 43), and short batches (700 x
+    2048 x 5504 "gate": 49 and 58)."""
     key = (kind, M, N, K)
     best = _PLANS.get(key)
     if best is None:
         steps = -(-K // 64)
-        for tile in range(len(_TILES)):
+        for tile in range(_DW_TILES if kind == "dw" else len(_TILES)):
             tiles = _count(tile, M, N)
             for splits in ((1, 2, 4, 8) if kind in ("down", "dx", "dw") else (1,)):
                 if splits > 1 and (tiles * splits > 256 or steps < 8 * splits):
                     break
-                est = _estimate(tile, tiles * splits, -(-steps // splits))
+                est = _estimate(tile, tiles * splits, -(-steps // splits), kind)
                 if splits > 1:                   # partials written and read, one more launch
                     est += 4.0 + splits * M * N * 8 / 4e6
                 if best is None or est < best[2]:
@@ -161,7 +168,7 @@ def _plan_pair(T, H, F, Ho):
     key = ("pair", T, H, F, Ho)
     if key not in _PLANS:
         best, cost = None, _plan("dw", 2 * F, H, T)[2] + _plan("dw", Ho, F, T)[2] + 2.0
-        for tile in range(len(_TILES)):
+        for tile in range(_DW_TILES):
             est = _estimate(tile, _count(tile, 2 * F, H) + _count(tile, Ho, F), -(-T // 64))
             if est < cost:
                 best, cost = tile, est

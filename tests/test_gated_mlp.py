@@ -328,3 +328,18 @@ def test_gpu_few_tokens_of_wide_features(T):
     y, pre, h = ops.gated_mlp_fwd(x, w1, b1, w2, b2)
     _within(y, _oracle("silu", x, w1, b1, w2, b2)["y"], "y")
     assert torch.equal(ops.gated_mlp_fwd(x, w1, b1, w2, b2, save=False)[0], y)
+
+
+@gpu
+@pytest.mark.parametrize("tile", range(6))
+@pytest.mark.parametrize("T,H,F,Ho", [(70, 72, 136, 40), (333, 264, 200, 392), (1003, 768, 520, 256)])
+def test_gpu_every_tile(monkeypatch, T, H, F, Ho, tile):
+    """Any tile may be chosen for a shape: all of them, where they are taken, give the block's results."""
+    import mxtrain.ops.gated as gated
+    plan = gated._plan
+    monkeypatch.setattr(gated, "_plan", lambda kind, *a: plan(kind, *a) if kind == "dw" else (tile, 1, 0.0))
+    x, w1, b1, w2, b2, dy = _make(T, H, F, Ho, True, seed=T, device=DEV)
+    y, pre, h = ops.gated_mlp_fwd(x, w1, b1, w2, b2, "gelu")
+    got = dict(zip(("dx", "dw1", "db1", "dw2", "db2"), ops.gated_mlp_bwd(dy, x, pre, h, w1, b1, w2, b2, "gelu")), y=y)
+    for name, want in _oracle("gelu", x, w1, b1, w2, b2, dy).items():
+        _within(got[name], want, name)
