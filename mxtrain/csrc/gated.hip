@@ -653,33 +653,34 @@ MX_EXPORT int mx_gated_tile(int tile, int what) {
   return what == 0 ? kTiles[tile].bm : what == 1 ? kTiles[tile].bn : kTiles[tile].wm;
 }
 
-// h[M][F] = act(x W1a^T + b1a) (x W1b^T + b1b): x [M][ldx] (K wide), w1 [2F][ldw]; pre [M][2F] or null
-MX_EXPORT int mx_gated_fwd(const void* x, int ldx, const void* w1, int ldw, const void* b1, void* pre, void* h, int M,
-                           int K, int F, int act, int tile, hipStream_t s) {
-  if (M <= 0 || bad_dim(K) || bad_dim(F) || bad_rows(x, ldx, K) || bad_rows(w1, ldw, K) || bad_rows(h, F, F) ||
-      ((uintptr_t)pre & 15) || ((uintptr_t)b1 & 15) || act < 0 || act > 1)
+// whether M tokens take the few-token form in a product of K x N weights (no tile, no splits)
+MX_EXPORT int mx_gated_few(int M, int K, int N) {
+  GArgs g{};
+  g.M = M; g.N = N; g.K = K;
+  return few_tokens(g);
+}
+
+// h[M][F] = act(x W1a^T + b1a) (x W1b^T + b1b), y[M][Ho] = h W2^T + b2: x [M][ldx] (H wide), w1 [2F][ld1], w2
+// [Ho][ld2], biases or null; pre [M][2F] or null; part: splits x M x Ho floats (splits > 1)
+MX_EXPORT int mx_gated_fwd(const void* x, int ldx, const void* w1, int ld1, const void* b1, void* pre, void* h,
+                           const void* w2, int ld2, const void* b2, void* y, int M, int H, int F, int Ho, int act,
+                           int gate_tile, int down_tile, int splits, float* part, hipStream_t s) {
+  if (M <= 0 || bad_dim(H) || bad_dim(F) || bad_dim(Ho) || bad_rows(x, ldx, H) || bad_rows(w1, ld1, H) ||
+      bad_rows(h, F, F) || bad_rows(w2, ld2, F) || bad_rows(y, Ho, Ho) || ((uintptr_t)pre & 15) ||
+      ((uintptr_t)b1 & 15) || ((uintptr_t)b2 & 15) || act < 0 || act > 1)
     return hipErrorInvalidValue;
   GArgs g{};
   g.a = (const uint16_t*)x; g.b = (const uint16_t*)w1; g.c = (uint16_t*)h; g.aux = (uint16_t*)pre;
   g.bias = (const uint16_t*)b1;
-  g.lda = ldx; g.ldb = ldw; g.ldc = F;
-  g.M = M; g.N = F; g.K = K; g.act = act;
-  if (few_tokens(g)) return run_few<true>(g, s);
-  return run<true, true, 2>(tile, 1, g, s);
-}
-
-// y[M][N] = h W2^T (+ b2): h [M][K] contiguous, w2 [N][ldw]; part: splits x M x N floats (splits > 1)
-MX_EXPORT int mx_gated_down(const void* h, const void* w2, int ldw, const void* b2, void* y, int M, int N, int K,
-                            int tile, int splits, float* part, hipStream_t s) {
-  if (M <= 0 || bad_dim(K) || bad_dim(N) || bad_rows(h, K, K) || bad_rows(w2, ldw, K) || bad_rows(y, N, N) ||
-      ((uintptr_t)b2 & 15))
-    return hipErrorInvalidValue;
-  GArgs g{};
-  g.a = (const uint16_t*)h; g.b = (const uint16_t*)w2; g.c = (uint16_t*)y; g.bias = (const uint16_t*)b2;
-  g.lda = K; g.ldb = ldw; g.ldc = N; g.part = part;
-  g.M = M; g.N = N; g.K = K;
-  if (few_tokens(g)) return run_few<false>(g, s);
-  return run<true, true, 1>(tile, splits, g, s);
+  g.lda = ldx; g.ldb = ld1; g.ldc = F;
+  g.M = M; g.N = F; g.K = H; g.act = act;
+  if (const int e = few_tokens(g) ? run_few<true>(g, s) : run<true, true, 2>(gate_tile, 1, g, s); e != hipSuccess)
+    return e;
+  GArgs d{};
+  d.a = (const uint16_t*)h; d.b = (const uint16_t*)w2; d.c = (uint16_t*)y; d.bias = (const uint16_t*)b2;
+  d.lda = F; d.ldb = ld2; d.ldc = Ho; d.part = part;
+  d.M = M; d.N = Ho; d.K = F;
+  return few_tokens(d) ? run_few<false>(d, s) : run<true, true, 1>(down_tile, splits, d, s);
 }
 
 // dpre[M][2F] = [dh b act'(a) | dh act(a)], dh = dy W2: dy [M][lddy] (K wide), w2 [K][ldw]; part null or

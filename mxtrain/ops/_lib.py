@@ -125,8 +125,8 @@ SIGNATURES = {
     "mx_embedding_bwd": [P, I64, P, I, P, I, I, I, F, I, P, I64, P],
     # gated.hip
     "mx_gated_tile": [I, I],
-    "mx_gated_fwd": [P, I, P, I, P, P, P, I, I, I, I, I, P],
-    "mx_gated_down": [P, P, I, P, P, I, I, I, I, I, P, P],
+    "mx_gated_few": [I, I, I],
+    "mx_gated_fwd": [P, I, P, I, P, P, P, P, I, P, P, I, I, I, I, I, I, I, I, P, P],
     "mx_gated_dgate": [P, I, P, I, P, P, P, I, I, I, I, I, P],
     "mx_gated_dx": [P, P, I, P, I, I, I, I, I, P, P],
     "mx_gated_dw": [P, I, P, I, P, I, I, I, I, I, I, I, P, P],

@@ -146,8 +146,10 @@ def _plan(kind, M, N, K):
     key = (kind, M, N, K)
     best = _PLANS.get(key)
     if best is None:
+        if kind in ("gate", "down") and _lib.query("mx_gated_few", M, K, N // 2 if kind == "gate" else N):
+            best = (0, 1, 0.0)       # (not looked at)
         steps = -(-K // 64)
-        for tile in range(_DW_TILES if kind == "dw" else len(_TILES)):
+        for tile in range(0 if best else _DW_TILES if kind == "dw" else len(_TILES)):
             tiles = _count(tile, M, N)
             for splits in ((1, 2, 4, 8) if kind in ("down", "dx", "dw") else (1,)):
                 if splits > 1 and (tiles * splits > 256 or steps < 8 * splits):
@@ -209,13 +211,10 @@ def gated_mlp_fwd(x, w1, b1, w2, b2, act: str = "silu", save: bool = True):
         y = torch.empty(T, Ho, dtype=x.dtype, device=x.device)
         h = torch.empty(T, F, dtype=x.dtype, device=x.device)
         pre = torch.empty(T, 2 * F, dtype=x.dtype, device=x.device) if save else None
-        s = _lib.stream()
-        _lib.call("mx_gated_fwd", x_, ldx, w1_, ld1, b1_, _lib.ptr(pre), h.data_ptr(), T, H, F, ACTS[act],
-                  _plan("gate", T, 2 * F, H)[0], s)
         tile, splits, _ = _plan("down", T, Ho, F)
         part = _split_ws(splits, T, Ho, x.device)
-        _lib.call("mx_gated_down", h.data_ptr(), w2_, ld2, b2_, y.data_ptr(), T, Ho, F, tile, splits, _lib.ptr(part),
-                  s)
+        _lib.call("mx_gated_fwd", x_, ldx, w1_, ld1, b1_, _lib.ptr(pre), h.data_ptr(), w2_, ld2, b2_, y.data_ptr(), T,
+                  H, F, Ho, ACTS[act], _plan("gate", T, 2 * F, H)[0], tile, splits, _lib.ptr(part), _lib.stream())
     return (y, pre, h) if save else (y, None, None)
 
 
