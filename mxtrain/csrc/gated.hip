@@ -10,6 +10,10 @@
 // without another pass.  dh never exists in memory: the epilogue of dy W2 reads a and b and
 // writes da, db and the column partials of the bias gradient.
 //
+// Rounded to bf16 on the way, once each from fp32: pre and h (what backward is given; fp32 would double the
+// largest tensors of the block) and [da | db] (a matrix operand of dx and dW1; its column sums are taken
+// before the rounding).  Splits, partial and column sums stay fp32.
+//
 // All six products share one kernel.  Operands are staged by LDS-DMA through buffer resources:
 // what lies past a tile's rows reads zero, so any number of tokens and any feature count that is a
 // multiple of 8 is taken without padding.  16 x 16 x 32 MFMA with the weight (column) operand

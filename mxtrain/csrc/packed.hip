@@ -220,10 +220,10 @@ __device__ __forceinline__ int pair_rank(int rank, int n) {
 // K / V tiles of BK keys arrive by LDS-DMA into a two-slot ring, one barrier per tile.  Two workgroups a
 // CU, so that one's exponentials run beside the other's products: 16384 tokens in one, 32 heads of 128,
 // forward 2.4 ms (0.92 PFLOP/s), dQ 2.9 (1.13); 4096 of ~300, 16 heads of 64, bound by the latency of a
-// block's few tiles, 20 and 23 us.
-template <int D, bool DQ>
+// block's few tiles, 20 and 23 us.  HALF: 64 rows, two waves for each 32 (see launch_qmajor).
+template <int D, bool DQ, bool HALF>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void packed_qmajor_kernel(const PArgs a) {
-  constexpr int BQ = 128, BK = D == 64 ? 128 : 64, NSUB = BK / 32, NKK = D / 16, NDT = D / 32;
+  constexpr int BQ = HALF ? 64 : 128, BK = D == 64 ? 128 : 64, NSUB = BK / 32, NKK = D / 16, NDT = D / 32;
   constexpr int RB = D * 2, CPR = D / 8, RPP = 64 / CPR, TILE = BK * RB, PPW = TILE / 1024 / 4;
   __shared__ __attribute__((aligned(16))) char kbuf0[TILE];
   __shared__ __attribute__((aligned(16))) char kbuf1[TILE];
@@ -231,17 +231,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ __attribute__((aligned(16))) char vbuf1[TILE];
   const int tid = threadIdx.x, lane = tid & 63, wl = uni(tid >> 6);
   const int r = lane & 31, hh = lane >> 5, g = lane >> 4, gi = lane & 15;
-  const int T = a.T, nqb = (T + BQ - 1) / BQ;
+  const int wq = HALF ? wl & 1 : wl, kh = HALF ? wl >> 1 : 0;   // row group; half of a key tile's subtiles
+  const int T = a.T, nqb = (T + 127) / 128;
   int rank, hq;
   block_map(a.Hq, rank, hq);
   const int hk = hq / (a.Hq / a.Hkv);
-  const int q0 = uni(a.order[pair_rank(rank, nqb)]) * BQ;
-  const int qw = q0 + 32 * wl, qrow = qw + r;
+  int q0 = 0;
+  if constexpr (HALF) q0 = uni(a.order[rank >> 1]) * 128 + 64 * (rank & 1 ^ 1);
+  else q0 = uni(a.order[pair_rank(rank, nqb)]) * 128;
+  const int qw = q0 + 32 * wq, qrow = qw + r;
   uint16_t* outp = a.out + (size_t)qrow * a.ldout + hq * D;
   // the table reads depend on nothing but the block (a row behind the last sequence has start = itself)
   const int nv = uni(a.meta[0]);
   const int qrow_c = min(qrow, T - 1);
-  const int kv_lo = uni(a.start[q0]) & ~31;
+  const int kv_lo = uni(a.start[min(q0, T - 1)]) & ~31;
   const int smin = uni(a.start[min(qw, T - 1)]), smax = uni(a.start[min(qw + 31, T - 1)]);
   const int st = a.start[qrow_c];
   if (q0 >= nv) {                                    // behind the last sequence
@@ -302,7 +305,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
       dl = xhalf_sum(s);
       lse2 = a.lse[(size_t)hq * T + qrow_c];
-      if (hh == 0 && qrow < nv) {   // what the dK / dV kernel starts its products from
+      if (hh == 0 && kh == 0 && qrow < nv) {   // what the dK / dV kernel starts its products from
         a.delta[(size_t)hq * T + qrow] = -dl;
         a.nlse[(size_t)hq * T + qrow] = -lse2 / a.c;
       }
@@ -450,17 +453,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
     }
   };
+  constexpr int NW = HALF ? NSUB / 2 : NSUB;   // subtiles of a tile for each wave
   auto compute = [&](const char* Kt, const char* Vt, int j) __attribute__((always_inline)) {
     const int k0 = kv_lo + j * BK;
     if (uni(!wave_on || k0 > wlast || k0 + BK <= smin ? 1 : 0)) return;
     if constexpr (!DQ) {   // whole tile visible to every row of the wave: straight-line code
       if (uni(k0 >= smax && k0 + BK <= qw + 1 && qw + 31 < nv ? 1 : 0)) {
-        block(Kt, Vt, k0, std::integral_constant<int, NSUB>{}, std::false_type{});
+        block(Kt + kh * NW * 32 * RB, Vt + kh * NW * 32 * RB, k0 + 32 * kh * NW, std::integral_constant<int, NW>{},
+              std::false_type{});
         return;
       }
     }
-    int t = max(0, (smin - k0) >> 5);
-    const int tb = min(NSUB - 1, (wlast - k0) >> 5);
+    int t = max(kh * NW, (smin - k0) >> 5);
+    const int tb = min(kh * NW + NW - 1, (wlast - k0) >> 5);
 #pragma unroll 1
     for (; t < tb; t += 2)
       block(Kt + 32 * t * RB, Vt + 32 * t * RB, k0 + 32 * t, std::integral_constant<int, 2>{}, std::true_type{});
@@ -478,6 +483,39 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if (j + 1 < ntile) step(kbuf1, vbuf1, kbuf0, vbuf0, j + 1);
   }
 
+  if constexpr (HALF) {   // the halves meet: m, l and the first columns in one buffer, the rest in the other
+    __syncthreads();
+    float* x = reinterpret_cast<float*>(wq ? kbuf1 : kbuf0) + lane;
+    float* y = reinterpret_cast<float*>(wq ? vbuf1 : vbuf0) + lane;
+    if (kh == 1) {
+      x[0] = m_i;
+      x[64] = l_i;
+      x[128] = __any(bad != 0) ? 1.f : 0.f;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          (dt < NDT / 2 ? x + 64 * (3 + 16 * dt + e) : y + 64 * (16 * (dt - NDT / 2) + e))[0] = acc[dt][e];
+    }
+    __syncthreads();
+    if (kh == 1) return;
+    bad |= x[128] != 0.f;
+    float a0 = 1.f, a1 = 1.f;
+    if constexpr (!DQ) {
+      // (a half that saw no finite score holds sums of 0 or NaN, whatever their scale)
+      const float m1 = x[0], m = fmaxf(m_i, m1);
+      a0 = m_i == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_i - m) * c);
+      a1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m1 - m) * c);
+      l_i = l_i * a0 + x[64] * a1;
+      m_i = m;
+    }
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        acc[dt][e] = acc[dt][e] * a0 +
+                     (dt < NDT / 2 ? x + 64 * (3 + 16 * dt + e) : y + 64 * (16 * (dt - NDT / 2) + e))[0] * a1;
+  }
   if (a.fill && qrow >= nv && qrow < T) {
     zero_row<D>(outp, hh);
     if (!DQ && hh == 0) a.lse[(size_t)hq * T + qrow] = INFINITY;
@@ -1232,6 +1270,24 @@ int key_shares(int T, int Hq, int Hkv, int D) {
   return D == 128 && Hq > Hkv && blocks < 1024 && (int64_t)T * Hq >= 60000 ? 256 : 0;
 }
 
+// At most one block for each CU: 64-row blocks whose wave pairs take half of the keys each, which halves the
+// longest chain of tiles (2048 tokens in one, 16 heads of 64, forward 29.6 -> 24.7 us, of 128, 50 -> 42 and dQ + dK +
+// dV 140 -> 120; 512 tokens 12.2 -> 11.5 and 17.0 -> 14.2).  With more blocks the CUs are full without it and the
+// twice as many tiles cost more: 4096 of ~300, 16 heads of 64, 18.7 -> 20.2; 8000 of ~900, 32 heads of 128, 124 -> 151.
+template <bool DQ>
+int launch_qmajor(const PArgs& a, int D, hipStream_t s) {
+  const unsigned n = (unsigned)((a.T + 127) / 128 * a.Hq);
+  const bool half = n <= 256;
+  if (D == 64) {
+    if (half) hipLaunchKernelGGL((packed_qmajor_kernel<64, DQ, true>), dim3(2 * n), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((packed_qmajor_kernel<64, DQ, false>), dim3(n), dim3(256), 0, s, a);
+  } else {
+    if (half) hipLaunchKernelGGL((packed_qmajor_kernel<128, DQ, true>), dim3(2 * n), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((packed_qmajor_kernel<128, DQ, false>), dim3(n), dim3(256), 0, s, a);
+  }
+  return hipGetLastError();
+}
+
 bool bad_mat(const void* p, int ld, int width) {   // 16-B rows, tile offsets below 2^31 bytes
   return p == nullptr || ((uintptr_t)p & 15) || (ld & 7) || ld < width || ld > (1 << 22);
 }
@@ -1279,10 +1335,7 @@ MX_EXPORT int mx_packed_attn_fwd(const void* q, const void* k, const void* v, in
   a.c = scale * 1.4426950408889634f;
   a.scale = scale;
   a.fill = fill;
-  const dim3 grid((unsigned)((T + 127) / 128 * Hq));
-  if (D == 64) hipLaunchKernelGGL((packed_qmajor_kernel<64, false>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((packed_qmajor_kernel<128, false>), grid, dim3(256), 0, s, a);
-  return hipGetLastError();
+  return launch_qmajor<false>(a, D, s);
 }
 
 // floats of `part` (0: none)
@@ -1325,11 +1378,11 @@ MX_EXPORT int mx_packed_attn_bwd(const void* q, const void* k, const void* v, in
     return hipErrorInvalidValue;
   const unsigned nb = (unsigned)((T + 127) / 128);
   if (D == 64) {
-    hipLaunchKernelGGL((packed_qmajor_kernel<64, true>), dim3(nb * Hq), dim3(256), 0, s, a);
+    launch_qmajor<true>(a, D, s);
     a.order = order + nb;
     hipLaunchKernelGGL((packed_kmajor_kernel<64>), dim3(nb * Hkv * a.nsplit), dim3(256), 0, s, a);
   } else {
-    hipLaunchKernelGGL((packed_qmajor_kernel<128, true>), dim3(nb * Hq), dim3(256), 0, s, a);
+    launch_qmajor<true>(a, D, s);
     a.order = order + 2 * nb;
     const unsigned nk = (unsigned)((T + KB2 - 1) / KB2);
     if (a.nshare) {

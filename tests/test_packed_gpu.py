@@ -352,3 +352,37 @@ def test_results_over_operands_are_refused():
     for bad in ((b, c, c), (b, b, c), (o, b, c), (b, c, do), (b, k, c)):
         with pytest.raises(ValueError):
             ops.packed_attn_bwd(do, q, k, v, o, lse, s, H, H, D, dq=bad[0], dk=bad[1], dv=bad[2])
+
+
+@pytest.mark.parametrize("lens,pad,Hq,Hkv", [([1200, 900], 31, 32, 32), ([40] * 50, 0, 32, 4), ([2048], 0, 17, 17),
+                                             ([1, 2047], 1, 16, 16)])
+def test_many_blocks_of_narrow_heads(lens, pad, Hq, Hkv):
+    """More query blocks than CUs (whole 128-row blocks), and just as many (halved ones)."""
+    D, T = 64, sum(lens) + pad
+    nv = T - pad
+    q, k, v, do = _inputs(T, Hq, Hkv, D, seed=41)
+    s = ops.pack_sequences(_cu(lens), T, device=DEV)
+    want = attention(q, k, v, lens, Hq, Hkv, D, D ** -0.5, do)
+    for t in (q, k, v, do):
+        t[nv:] = float("inf")
+    o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D)
+    for name, t in zip(("o", "dq", "dk", "dv"), (o, *ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D))):
+        within(t[:nv], tuple(x[:nv] for x in want[name]), name)
+        assert (t[nv:] == 0).all(), name
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("-inf")])
+@pytest.mark.parametrize("D,H,lens", [(64, 32, [700, 800]), (64, 4, [700, 800]), (128, 4, [700, 800])])
+def test_non_finite_values_in_either_form(D, H, lens, bad):
+    T = sum(lens)
+    q, k, v, do = _inputs(T, H, H, D, seed=42)
+    s = ops.pack_sequences(_cu(lens), T, device=DEV)
+    want = attention(q, k, v, lens, H, H, D, D ** -0.5, do)
+    for t in (q, k, v, do):
+        t[690:700] = bad
+    o, lse = ops.packed_attn_fwd(q, k, v, s, H, H, D)
+    grads = ops.packed_attn_bwd(do, q, k, v, o, lse, s, H, H, D)
+    for name, t in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+        within(t[700:], tuple(x[700:] for x in want[name]), name)
+    within(o[:690], tuple(x[:690] for x in want["o"]), "o")
+    within(grads[0][:690], tuple(x[:690] for x in want["dq"]), "dq")
