@@ -20,7 +20,7 @@
 // first, so that a lane holds 4 consecutive columns of a row.
 //
 // Large products are bound by their K loop: at 128 x 64 a wave the fragment reads from LDS take as long
-// as the matrix pipe (1.1 - 1.25 PFLOP/s; forward and backward of 4096 x 4096 x 10880 in 2.95 ms).  Short
+// as the matrix pipe (1.1 - 1.25 PFLOP/s; forward and backward of 4096 x 4096 x 10880 in 3.0 ms).  Short
 // ones (4096 x 1024 x 2688: 0.27 ms) by rounds of workgroups that fill and drain for 16 - 84 steps.
 #include "gemm_common.h"
 

@@ -219,7 +219,7 @@ __device__ __forceinline__ int pair_rank(int rank, int n) {
 // (S^T = K Q^T, O^T = V^T P^T), so the softmax statistics are lane-local plus one half exchange.
 // K / V tiles of BK keys arrive by LDS-DMA into a two-slot ring, one barrier per tile.  Two workgroups a
 // CU, so that one's exponentials run beside the other's products: 16384 tokens in one, 32 heads of 128,
-// forward 2.4 ms (0.92 PFLOP/s), dQ 2.9 (1.13); 4096 of ~300, 16 heads of 64, bound by the latency of a
+// forward 2.15 ms (1.03 PFLOP/s), dQ 2.95 (1.12); 4096 of ~300, 16 heads of 64, bound by the latency of a
 // block's few tiles, 20 and 23 us.  HALF: 64 rows, two waves for each 32 (see launch_qmajor).
 template <int D, bool DQ, bool HALF>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void packed_qmajor_kernel(const PArgs a) {
