@@ -584,9 +584,11 @@ __device__ __forceinline__ int block_splits(const PArgs& a, int items) {
 
 // D = 128, few key blocks: the items of all of them, head by head and block by block, are one line that
 // is cut into even shares, one per workgroup; a block that a cut falls into is done in pieces, whose
-// fp32 sums packed_join2_kernel adds.  A block costs PIECE items beside its own (its K and V rows, its
-// results), a piece about SNAP (its partial sums): a cut nearer to the end of a block moves there.
-constexpr int PIECE = 2, SNAP = 5, SHARE_MIN = 8;
+// fp32 sums packed_join2_kernel adds.  A block counts PIECE items beside its own (its K and V rows, its
+// results); a cut within SNAP items of a block's end moves there.  (Moving cuts saves partial sums but makes
+// shares uneven: 4096 tokens of ~300, 16 / 4 heads, dQ + dK + dV 153 us in the mean of three batches at 2, 163 at
+// 5, 224 at 16.)
+constexpr int PIECE = 3, SNAP = 2, SHARE_MIN = 8;
 __device__ __forceinline__ int64_t uni64(int64_t x) {
   return (int64_t)((uint64_t)(uint32_t)uni((int)x) | (uint64_t)(uint32_t)uni((int)(x >> 32)) << 32);
 }
@@ -1274,10 +1276,12 @@ int key_shares(int T, int Hq, int Hkv, int D) {
 // longest chain of tiles (2048 tokens in one, 16 heads of 64, forward 29.6 -> 24.7 us, of 128, 50 -> 42 and dQ + dK +
 // dV 140 -> 120; 512 tokens 12.2 -> 11.5 and 17.0 -> 14.2).  With more blocks the CUs are full without it and the
 // twice as many tiles cost more: 4096 of ~300, 16 heads of 64, 18.7 -> 20.2; 8000 of ~900, 32 heads of 128, 124 -> 151.
+// Up to two for the forward of 128, whose half blocks need no spilled registers (4096 in one, 16 heads, 101 -> 96 us;
+// 2048 of ~300, 32 heads, 32 -> 28; dQ + dK + dV of 2048 in one, 32 heads, 190 -> 197).
 template <bool DQ>
 int launch_qmajor(const PArgs& a, int D, hipStream_t s) {
   const unsigned n = (unsigned)((a.T + 127) / 128 * a.Hq);
-  const bool half = n <= 256;
+  const bool half = n <= (D == 128 && !DQ ? 512 : 256);
   if (D == 64) {
     if (half) hipLaunchKernelGGL((packed_qmajor_kernel<64, DQ, true>), dim3(2 * n), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((packed_qmajor_kernel<64, DQ, false>), dim3(n), dim3(256), 0, s, a);
