@@ -20,8 +20,8 @@
 // first, so that a lane holds 4 consecutive columns of a row.
 //
 // Large products are bound by their K loop: at 128 x 64 a wave the fragment reads from LDS take as long
-// as the matrix pipe (1.1 - 1.25 PFLOP/s; forward and backward of 4096 x 4096 x 10880 in 3.0 ms).  Short
-// ones (4096 x 1024 x 2688: 0.27 ms) by rounds of workgroups that fill and drain for 16 - 84 steps.
+// as the matrix pipe (1.1 - 1.25 PFLOP/s; forward and backward of 4096 x 4096 x 10880 in 2.9 ms).  Short
+// ones (4096 x 1024 x 2688: 0.26 ms) by rounds of workgroups that fill and drain for 16 - 84 steps.
 #include "gemm_common.h"
 
 #include <type_traits>
@@ -605,12 +605,11 @@ struct Tile {
   int bm, bn, wm;
 };
 constexpr Tile kTiles[] = {
-    {128, 128, 2},   // 0: 4 waves of 64 x 64, 64-deep steps, 2 slots: two workgroups per CU
-    {256, 256, 2},   // 1: 8 waves of 128 x 64, 64-deep steps, 2 slots
-    {256, 256, 2},   // 2: 8 waves of 128 x 64, 32-deep steps, 4 slots
-    {128, 128, 4},   // 3: 8 waves of 32 x 64, 64-deep steps, 4 slots
-    {256, 128, 4},   // 4: 8 waves of 64 x 64, 64-deep steps, 3 slots
-    {64, 128, 2},    // 5: 4 waves of 32 x 64, 64-deep steps, 3 slots (not for weight gradients)
+    {128, 128, 2},   // 0: 4 waves of 64 x 64, 64-deep steps, 2 slots, two workgroups per CU
+    {256, 256, 2},   // 1: 8 waves of 128 x 64, 32-deep steps, 4 slots
+    {128, 128, 4},   // 2: 8 waves of 32 x 64, 64-deep steps, 4 slots
+    {256, 128, 4},   // 3: 8 waves of 64 x 64, 64-deep steps, 3 slots
+    {64, 128, 2},    // 4: 4 waves of 32 x 64, 64-deep steps, 3 slots, two per CU (not for weight gradients)
 };
 constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
 
@@ -618,11 +617,10 @@ template <bool AKC, bool BKC, int EPI>
 int run_tile(int tile, const GArgs& g, hipStream_t s) {
   switch (tile) {
     case 0: return launch<AKC, BKC, 2, 2, 4, 4, 64, 2, EPI>(g, s);
-    case 1: return launch<AKC, BKC, 2, 4, 8, 4, 64, 2, EPI>(g, s);
-    case 2: return launch<AKC, BKC, 2, 4, 8, 4, 32, 4, EPI>(g, s);
-    case 3: return launch<AKC, BKC, 4, 2, 2, 4, 64, 4, EPI>(g, s);
-    case 4: return launch<AKC, BKC, 4, 2, 4, 4, 64, 3, EPI>(g, s);
-    case 5:
+    case 1: return launch<AKC, BKC, 2, 4, 8, 4, 32, 4, EPI>(g, s);
+    case 2: return launch<AKC, BKC, 4, 2, 2, 4, 64, 4, EPI>(g, s);
+    case 3: return launch<AKC, BKC, 4, 2, 4, 4, 64, 3, EPI>(g, s);
+    case 4:
       if constexpr (AKC) return launch<AKC, BKC, 2, 2, 2, 4, 64, 3, EPI>(g, s);
       return hipErrorInvalidValue;
     default: return hipErrorInvalidValue;

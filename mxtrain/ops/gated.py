@@ -113,10 +113,10 @@ def _mats(act, x, w1, b1, w2, b2):
 # steps, more of it where the epilogue reads and writes as much as the gate gradient's, and once.
 # Fitted to one MI355X over 4096 x 4096 x 10880 (steps), 4096 x 1024 x 2688 (rounds) and, the small
 # tile, 1003 x 768 x 2048 and 300 x 512 x 1376.
-_TILES = ((128, 128, 2, 1.14, 0.97, 5.0, 3.5, 0.0), (256, 256, 1, 1.69, 1.69, 8.0, 33.0, 0.0),
-          (256, 256, 1, 1.72, 1.72, 5.0, 30.0, 0.0), (128, 128, 1, 0.62, 0.62, 4.0, 4.2, 0.0),
+_TILES = ((128, 128, 2, 1.14, 0.97, 5.0, 3.5, 0.0), (256, 256, 1, 1.72, 1.72, 5.0, 30.0, 0.0),
+          (128, 128, 1, 0.62, 0.62, 4.0, 4.2, 0.0),
           (256, 128, 1, 0.985, 0.985, 5.0, 7.5, 0.0), (64, 128, 2, 0.57, 0.45, 2.5, 3.6, 6.0))
-_DW_TILES = 5          # (the last one does not take operands whose rows are the contraction)
+_DW_TILES = 4          # (the last one does not take operands whose rows are the contraction)
 _PLANS = {}
 
 
@@ -136,7 +136,7 @@ def _count(tile, M, N):
 def _plan(kind, M, N, K):
     """(tile, splits, us) of one product, M x N over K (N: columns of both halves for "gate"): the
     least estimated time.  Big tiles move the fewest operand bytes per product, so they win where
-    they fill whole rounds (4096 x 4096 x 10880 "down": 287 us with 256 x 256 tiles, 387 with 128 x
+    they fill whole rounds (4096 x 4096 x 10880 "down": 298 us with 256 x 256 tiles, 387 with 128 x
     128); few tiles leave CUs idle, so smaller ones with a deeper ring win (1003 x 768 x 2048 "gate":
     12.6 us against 24.9), and a long K is split once the tiles cover less than half of the chip
     (its "dx": 21.2 us in 4 splits, 40 us in one).  Tiles of 64 rows, two workgroups a CU, run one's
