@@ -6,7 +6,7 @@ The two projections, the activation and the product are one kernel; backward rec
 but the activation: it needs the ``pre`` and ``h`` that forward saves.  W1 is [2F, H] with the gate
 half first (the layout of ``bias_swiglu_fwd`` and the GPT model's fc1), W2 [Ho, F].
 
-On the GPU: bfloat16, feature counts that are multiples of 8, any number of tokens; rows may be
+On the GPU: bfloat16, feature counts that are multiples of 8, up to 1048560 tokens; rows may be
 strided.  Products accumulate in fp32; ``pre``, ``h`` and every result are rounded once to bf16.
 """
 from __future__ import annotations
