@@ -575,11 +575,17 @@ constexpr int KB1 = 128, KB2 = 256, QT2 = 64;   // keys of a block (D = 64 / 128
 // for its partial sums.  dQ, dK, dV of 8 query heads on one key head, 512 tokens: 73 -> 38 us (D 64),
 // 156 -> 65 us (D 128); without the extra items 4096 tokens of ~300-token documents take 120 us, not 99
 // (16 heads of 128); with shares twice as large 16384 tokens, 16 / 4 heads, take 4.9 ms, not 3.8.
+// No split is empty (the last would fetch rows and statistics behind the last query head): 88 items in 16
+// splits of 6 are 15.
+__host__ __device__ inline int split_count(int64_t tiles, int Hq, int D, int nsplit, int items) {
+  if (nsplit == 1) return 1;
+  const int64_t share = tiles * Hq / (D == 64 ? 512 : 256) + 5, most = (items + share - 1) / share;
+  const int n = most < 1 ? 1 : most < nsplit ? (int)most : nsplit, per = (items + n - 1) / n;
+  return (items + per - 1) / per;
+}
 template <int D>
 __device__ __forceinline__ int block_splits(const PArgs& a, int items) {
-  const int64_t even = (D == 64 ? (int64_t)a.meta[1] : a.before[(a.T + KB2 - 1) / KB2]) * a.Hq / (D == 64 ? 512 : 256);
-  const int share = (int)min(even, (int64_t)1 << 30) + 5;
-  return max(1, min(a.nsplit, (items + share - 1) / share));
+  return split_count(D == 64 ? (int64_t)a.meta[1] : a.before[(a.T + KB2 - 1) / KB2], a.Hq, D, a.nsplit, items);
 }
 
 // D = 128, few key blocks: the items of all of them, head by head and block by block, are one line that
@@ -1340,6 +1346,12 @@ MX_EXPORT int mx_packed_attn_fwd(const void* q, const void* k, const void* v, in
   a.scale = scale;
   a.fill = fill;
   return launch_qmajor<false>(a, D, s);
+}
+
+// splits of a key block of `items` (query head, query tile) pairs in a batch of `tiles` query tiles; 0: none (shares)
+MX_EXPORT int mx_packed_block_splits(int T, int Hq, int Hkv, int D, int64_t tiles, int items) {
+  if (bad_shape(T, Hq, Hkv, D) || tiles < 0 || items < 1 || key_shares(T, Hq, Hkv, D)) return 0;
+  return split_count(tiles, Hq, D, key_splits(T, Hq, Hkv, D), items);
 }
 
 // floats of `part` (0: none)

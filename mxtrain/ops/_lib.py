@@ -117,6 +117,7 @@ SIGNATURES = {
     "mx_packed_plan": [P, I, I, I, P, P, P, P, P, P],
     "mx_packed_order_len": [I],
     "mx_packed_attn_fwd": [P, P, P, I, I, I, P, I, P, P, P, P, P, I, I, I, I, F, I, P],
+    "mx_packed_block_splits": [I, I, I, I, I64, I],
     "mx_packed_attn_bwd_floats": [I, I, I, I],
     "mx_packed_attn_bwd": [P, P, P, I, I, I, P, I, P, I, P, P, P, I, P, P, I, I, P, P, P, P, I, I, I, I, F, I, P, I64, P],
     # embedding.hip

@@ -105,3 +105,29 @@ def test_overlap_of_strided_matrices():
     assert not _lib.overlap(10, m(a), m(b)) and not _lib.overlap(10, m(b), m(a))
     assert _lib.overlap(10, m(a), m(a)) and _lib.overlap(10, m(a), (a.data_ptr() + 64, 200, 8))
     assert not _lib.overlap(10, m(buf), m(torch.zeros(10, 96, dtype=torch.bfloat16)))
+
+
+@pytest.mark.parametrize("D,kb", [(64, 128), (128, 256)])
+@pytest.mark.parametrize("heads", [(8, 1), (4, 1), (16, 4), (32, 8), (20, 5), (12, 12), (16, 16)])
+def test_no_split_of_a_key_block_is_empty(heads, D, kb):
+    """Every split of a key block begins at one of its (query head, query tile) items: one that did not
+    would fetch the rows and statistics of a query head that is not there.  (Lengths of one document, and
+    the first of two, up to where blocks are no longer split.)"""
+    from mxtrain.ops import _lib
+    Hq, Hkv = heads
+    split = set()
+    for T in (*range(1, 2200, 7), *range(640, 1605, 64), *range(2200, 20000, 411)):
+        for n in {T, max(1, T // 3)}:
+            ends = [n if k < n else T for k in range(0, T, kb)]
+            per_block = [-(-(max(e, min(k + kb, T)) - k) // 64) for e, k in zip(ends, range(0, T, kb))]
+            tiles = sum(per_block)
+            for q in set(per_block):
+                items = q * (Hq // Hkv)
+                nsp = _lib.query("mx_packed_block_splits", T, Hq, Hkv, D, tiles, items)
+                if nsp == 0:       # (cut into even shares)
+                    continue
+                assert 1 <= nsp <= 16
+                per = -(-items // nsp)
+                assert (nsp - 1) * per < items, (T, n, items, nsp)
+                split.add(nsp)
+    assert split

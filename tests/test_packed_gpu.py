@@ -386,3 +386,16 @@ def test_non_finite_values_in_either_form(D, H, lens, bad):
         within(t[700:], tuple(x[700:] for x in want[name]), name)
     within(o[:690], tuple(x[:690] for x in want["o"]), "o")
     within(grads[0][:690], tuple(x[:690] for x in want["dq"]), "dq")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens", [[700], [1541], [641, 5]])
+def test_one_key_head_of_one_document(lens, D):
+    """Key blocks cut into the most splits, where a whole number of items does not divide among them."""
+    Hq, Hkv, T = 8, 1, sum(lens)
+    q, k, v, do = _inputs(T, Hq, Hkv, D, seed=51)
+    s = ops.pack_sequences(_cu(lens), T, device=DEV)
+    o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D)
+    want = attention(q, k, v, lens, Hq, Hkv, D, D ** -0.5, do)
+    for name, t in zip(("o", "dq", "dk", "dv"), (o, *ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D))):
+        within(t, want[name], name)
