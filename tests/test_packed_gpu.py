@@ -399,3 +399,24 @@ def test_one_key_head_of_one_document(lens, D):
     want = attention(q, k, v, lens, Hq, Hkv, D, D ** -0.5, do)
     for name, t in zip(("o", "dq", "dk", "dv"), (o, *ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D))):
         within(t, want[name], name)
+
+
+@pytest.mark.parametrize("D,heads,lens", [(64, (2, 2), [100, 90]), (64, (4, 1), [1300, 900]), (128, (2, 2), [100, 90]),
+                                          (128, (4, 1), [1300, 900]), (128, (16, 4), [1900, 2300])])
+@pytest.mark.parametrize("inside", [False, True])
+def test_large_finite_values_of_masked_pairs(D, heads, lens, inside):
+    """dout of the first rows and V of the last ones are so large that their products, which no row may see,
+    pass the fp32 range: on both sides of a border, and inside a document, where no earlier row sees a later
+    key."""
+    (Hq, Hkv), T = heads, sum(lens)
+    q, k, v, do = _inputs(T, Hq, Hkv, D, seed=61)
+    at = lens[0]
+    do[:at] *= 1e20
+    v[at:] *= 1e20
+    lens = [T] if inside else lens
+    s = ops.pack_sequences(_cu(lens), T, device=DEV)
+    want = attention(q, k, v, lens, Hq, Hkv, D, D ** -0.5, do)
+    o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D)
+    grads = ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D)
+    for name, t in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+        within(t, want[name], name)
