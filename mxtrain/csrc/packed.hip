@@ -1396,26 +1396,19 @@ MX_EXPORT int mx_packed_attn_bwd(const void* q, const void* k, const void* v, in
   a.part = part;
   if (const int64_t n = mx_packed_attn_bwd_floats(T, Hq, Hkv, D); n && (!part || ((uintptr_t)part & 15) || part_floats < n))
     return hipErrorInvalidValue;
-  const unsigned nb = (unsigned)((T + 127) / 128);
-  if (D == 64) {
-    launch_qmajor<true>(a, D, s);
-    a.order = order + nb;
+  if (const int e = launch_qmajor<true>(a, D, s); e != hipSuccess) return e;   // (dK / dV read its statistics)
+  const unsigned nb = (unsigned)((T + 127) / 128), nk = (unsigned)((T + KB2 - 1) / KB2);
+  a.order = order + (D == 64 ? nb : 2 * nb);
+  if (D == 64)
     hipLaunchKernelGGL((packed_kmajor_kernel<64>), dim3(nb * Hkv * a.nsplit), dim3(256), 0, s, a);
-  } else {
-    launch_qmajor<true>(a, D, s);
-    a.order = order + 2 * nb;
-    const unsigned nk = (unsigned)((T + KB2 - 1) / KB2);
-    if (a.nshare) {
-      hipLaunchKernelGGL((packed_kmajor2_kernel<128, true>), dim3(a.nshare), dim3(256), 0, s, a);
-      hipLaunchKernelGGL(packed_join2_kernel, dim3((a.nshare - 1) * JOIN), dim3(256), 0, s, a);
-      return hipGetLastError();
-    }
+  else if (a.nshare)
+    hipLaunchKernelGGL((packed_kmajor2_kernel<128, true>), dim3(a.nshare), dim3(256), 0, s, a);
+  else
     hipLaunchKernelGGL((packed_kmajor2_kernel<128, false>), dim3(nk * Hkv * a.nsplit), dim3(256), 0, s, a);
-  }
-  if (a.nsplit > 1) {
-    const dim3 grid((unsigned)(((int64_t)T * Hkv * (D / 4) + 255) / 256));
-    if (D == 64) hipLaunchKernelGGL((packed_join_kernel<64>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((packed_join_kernel<128>), grid, dim3(256), 0, s, a);
-  }
+  if (const int e = hipGetLastError(); e != hipSuccess || (!a.nshare && a.nsplit == 1)) return e;
+  const dim3 grid((unsigned)(((int64_t)T * Hkv * (D / 4) + 255) / 256));
+  if (a.nshare) hipLaunchKernelGGL(packed_join2_kernel, dim3((a.nshare - 1) * JOIN), dim3(256), 0, s, a);
+  else if (D == 64) hipLaunchKernelGGL((packed_join_kernel<64>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((packed_join_kernel<128>), grid, dim3(256), 0, s, a);
   return hipGetLastError();
 }
