@@ -370,21 +370,27 @@ MX_EXPORT int mx_embedding_bwd(const void* ids, int64_t vstart, const void* dout
   int *k0 = b, *i0 = b + t4, *k1 = b + 2 * t4, *i1 = b + 3 * t4, *hist = b + 4 * t4;
   float* part = (float*)(hist + (((int64_t)p.blocks << p.bits) + 3 & ~3ll));
   SortArgs a{(const int64_t*)ids, vstart, V, T, p.tpb, nullptr, nullptr, k0, i0, hist, 0, p.bits};
+  // (each launch is looked at before the next: the sums read at the token numbers that the sort writes)
+  hipError_t e = hipSuccess;
   if (T <= SMALL) {
     hipLaunchKernelGGL(sort_small_kernel, dim3((T + 15) / 16), dim3(SORT_NT), 0, s, a);
+    e = hipGetLastError();
     a.kin = k0;
     a.iin = i0;
   }
   const size_t lds = (size_t)SORT_NW * sizeof(int) << p.bits;
-  for (int q = 0; q < (T <= SMALL ? 0 : p.passes); ++q) {
+  for (int q = 0; q < (T <= SMALL ? 0 : p.passes) && e == hipSuccess; ++q) {
     a.shift = q * p.bits;
     hipLaunchKernelGGL(sort_hist_kernel, dim3(p.blocks), dim3(SORT_NT), 0, s, a);
+    if ((e = hipGetLastError()) != hipSuccess) break;
     hipLaunchKernelGGL(sort_scatter_kernel, dim3(p.blocks), dim3(SORT_NT), lds, s, a);
+    e = hipGetLastError();
     a.kin = a.kout;
     a.iin = a.iout;
     a.kout = a.kout == k0 ? k1 : k0;
     a.iout = a.iout == i0 ? i1 : i0;
   }
+  if (e != hipSuccess) return e;
   SumArgs u{a.kin, a.iin, (const uint16_t*)dout, (uint16_t*)table, part, T, V, H, ldd, (H + 511) / 512,
             (T + CH - 1) / CH, scale, accumulate};
   const int64_t items = (int64_t)u.chunks * u.ncol, sum_blocks = (items + 3) / 4;
@@ -392,7 +398,7 @@ MX_EXPORT int mx_embedding_bwd(const void* ids, int64_t vstart, const void* dout
   if (items >= ((int64_t)1 << 31) || sum_blocks + zero_blocks >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(embedding_sum_kernel, dim3((unsigned)(sum_blocks + zero_blocks)), dim3(256), 0, s, u,
                      (int)sum_blocks);
-  if (u.chunks > 1)
-    hipLaunchKernelGGL(embedding_join_kernel, dim3((unsigned)sum_blocks), dim3(256), 0, s, u);
+  if ((e = hipGetLastError()) != hipSuccess || u.chunks == 1) return e;
+  hipLaunchKernelGGL(embedding_join_kernel, dim3((unsigned)sum_blocks), dim3(256), 0, s, u);
   return hipGetLastError();
 }

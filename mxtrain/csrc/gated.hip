@@ -594,6 +594,7 @@ int launch(GArgs g, hipStream_t s) {
   hipLaunchKernelGGL((gated_gemm_kernel<AKC, BKC, WM, WN, FM, FN, BKT, NSLOT, 2, EPI>), dim3((unsigned)grid),
                      dim3(Gm::NT), 0, s, g);
   if (EPI == 4) {
+    if (const int e = hipGetLastError(); e != hipSuccess) return e;
     const int64_t vecs = (int64_t)g.M * (g.N / 8);
     hipLaunchKernelGGL(gated_join_kernel, dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, s, g);
   }

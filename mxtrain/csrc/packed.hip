@@ -1324,6 +1324,7 @@ MX_EXPORT int mx_packed_plan(const void* cu, int wide, int n, int T, int* start,
   else
     hipLaunchKernelGGL((packed_plan_kernel<int32_t>), grid, dim3(256), 0, s, (const int32_t*)cu, n, T, start, end,
                        meta, (int64_t*)pos);
+  if (const int e = hipGetLastError(); e != hipSuccess) return e;
   hipLaunchKernelGGL(packed_order_kernel, dim3(1), dim3(1024), 0, s, T, start, end, meta, order);
   return hipGetLastError();
 }

@@ -98,3 +98,32 @@ def test_packed_attention_backward(fake, T, Hq, Hkv, D, launches):
     assert ok[:2] == (0, launches) and len(failed) == launches
     for k, (err, n, _) in enumerate(failed):
         assert err != 0 and n == k + 1, (k, failed)
+
+
+@pytest.mark.parametrize("T,V,launches", [(31, 50, 2), (4096, 50304, 3), (40000, 50304, 6)])
+def test_embedding_gradient(fake, T, V, launches):
+    """Sums over unsorted (unwritten) token numbers would read anywhere."""
+    H, words = 64, _lib.query64("mx_embedding_bwd_words", T, V, 64)
+    ok, *failed = _launches(fake, "mx_embedding_bwd", A, 0, A, H, A, T, V, H, 1.0, 0, A, words, None)
+    assert ok[:2] == (0, launches) and len(failed) == launches
+    for k, (err, n, _) in enumerate(failed):
+        assert err != 0 and n == k + 1, (k, failed)
+
+
+def test_row_table(fake):
+    ok, *failed = _launches(fake, "mx_packed_plan", A, 1, 3, 1000, A, A, A, A, A, None)
+    assert ok[:2] == (0, 2) and [r[:2] for r in failed] == [(719, 1), (719, 2)]
+
+
+@pytest.mark.parametrize("T", [16, 1003])
+def test_gated_forward(fake, T):
+    ok, *failed = _launches(fake, "mx_gated_fwd", A, 768, A, 768, A, A, A, A, 2048, A, A, T, 768, 2048, 768, 0, 2, 2, 4, A,
+                            None)
+    assert ok[0] == 0 and len(failed) == ok[1] == (2 if T == 16 else 3)
+    for k, (err, n, _) in enumerate(failed):
+        assert err != 0 and n == k + 1, (k, failed)
+
+
+def test_gated_input_gradient(fake):
+    ok, *failed = _launches(fake, "mx_gated_dx", A, A, 768, A, 1003, 768, 4096, 2, 4, A, None)
+    assert ok[:2] == (0, 2) and [r[:2] for r in failed] == [(719, 1), (719, 2)]
