@@ -168,14 +168,16 @@ def _plan_pair(T, H, F, Ho):
     leave one round of workgroups unfilled, not two (4096 x 1024 x 2688: 64 us, apart 58 + 40; 4096 x
     4096 x 10880: 911 and 630 + 321; 2048 x 2048 x 5504 fills its rounds: 154 and 97 + 56)."""
     key = ("pair", T, H, F, Ho)
-    if key not in _PLANS:
+    plan = _PLANS.get(key)      # (one look: another thread may clear the table at any time)
+    if plan is None:
         best, cost = None, _plan("dw", 2 * F, H, T)[2] + _plan("dw", Ho, F, T)[2] + 2.0
         for tile in range(_DW_TILES):
             est = _estimate(tile, _count(tile, 2 * F, H) + _count(tile, Ho, F), -(-T // 64))
             if est < cost:
                 best, cost = tile, est
-        _keep(key, best)
-    return _PLANS[key]
+        plan = (best, cost)
+        _keep(key, plan)
+    return plan[0]
 
 
 def _keep(key, plan):

@@ -352,3 +352,22 @@ def test_gpu_tile_table_matches_the_kernels():
     for tile, row in enumerate(gated._TILES):
         assert (_lib.query("mx_gated_tile", tile, 0), _lib.query("mx_gated_tile", tile, 1)) == row[:2]
     assert _lib.query("mx_gated_tile", len(gated._TILES), 0) == -1
+
+
+def test_a_plan_is_returned_though_another_thread_clears_the_table(monkeypatch):
+    import mxtrain.ops.gated as gated
+    monkeypatch.setattr(gated, "_PLANS", {})
+    first = gated._plan_pair(1003, 768, 2048, 768), gated._plan("gate", 1003, 4096, 768)
+
+    class Cleared(dict):           # whatever is looked up is gone before it is looked up again
+        def __contains__(self, key):
+            found = super().__contains__(key)
+            self.clear()
+            return found
+
+        def __setitem__(self, key, value):
+            super().__setitem__(key, value)
+            self.clear()
+    for kept in ({}, dict(gated._PLANS)):
+        monkeypatch.setattr(gated, "_PLANS", Cleared(kept))
+        assert (gated._plan_pair(1003, 768, 2048, 768), gated._plan("gate", 1003, 4096, 768)) == first
