@@ -273,6 +273,30 @@ def overlap(T, a, b) -> bool:
     return lda != ldb or c < 2 * wa or c + 2 * wb > 2 * lda
 
 
+def lies_over(outs, ins) -> bool:
+    """Whether one of the tensors ``outs`` shares memory with another of them or with one of ``ins``
+    (column ranges of one buffer do not)."""
+    span = []
+    for t in (*outs, *ins):
+        p = t.data_ptr()
+        span.append((p, p + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+                     if t.numel() else p, t))
+    for i, (a0, a1, a) in enumerate(span[:len(outs)]):
+        for b0, b1, b in span[i + 1:]:
+            if a0 < b1 and b0 < a1 and not _columns_apart(a, b):
+                return True
+    return False
+
+
+def _columns_apart(a, b):
+    if a.dim() != 2 or a.stride() != b.stride() or a.stride(1) != 1 or a.stride(0) == 0 or a.dtype != b.dtype:
+        return False
+    if b.data_ptr() < a.data_ptr():
+        a, b = b, a
+    c, w = (b.data_ptr() - a.data_ptr()) // a.element_size() % a.stride(0), a.shape[1]
+    return c >= w and c + b.shape[1] <= a.stride(0)
+
+
 def rows_of(t, rows, cols, dev, ld_max):
     """(address, row stride) of a bfloat16 [rows, cols] matrix on device index ``dev`` that the
     kernels take in place -- unit column stride, 16-byte aligned rows that do not overlap -- or

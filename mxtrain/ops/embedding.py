@@ -112,10 +112,10 @@ def embedding_bwd(keys, dout, rows: int, scale: float = 1.0, out=None, accumulat
         raise ValueError(f"{name}: keys are on {keys.device}, dout on {dev}")
     if accumulate and out is None:
         raise ValueError(f"{name}: accumulate needs out")
-    if out is not None and T and out.data_ptr() == dout.data_ptr():
-        raise ValueError(f"{name}: out must not lie over dout")
     if out is not None:
         _check_table(name, "out", out, dev, H)
+        if T and _lib.lies_over((out,), (dout,)):
+            raise ValueError(f"{name}: out must not lie over dout")
         if out.shape[0] != rows or out.dtype != dout.dtype:
             raise ValueError(f"{name}: out must be [{rows}, {H}] of type {dout.dtype}")
     hip = _lib.use_hip(dout)

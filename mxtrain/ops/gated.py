@@ -239,9 +239,8 @@ def gated_mlp_bwd(dy, x, pre, h, w1, b1, w2, b2, act: str = "silu", dw1=None, db
         db1=(db1, lambda T, H, F, O: (2 * F,)), dw2=(dw2, lambda T, H, F, O: (O, F)),
         db2=(db2, lambda T, H, F, O: (O,)))
     if need_dw:
-        out = {t.data_ptr() for t in (dw1, db1, dw2, db2) if t is not None}
-        if T and (len(out) < sum(t is not None for t in (dw1, db1, dw2, db2))
-                  or out & {t.data_ptr() for t in (dy, x, pre, h)}):
+        out = [t for t in (dw1, db1, dw2, db2) if t is not None]
+        if T and out and _lib.lies_over(out, (dy, x, pre, h)):
             raise ValueError(f"{name}: gradient buffers must not lie over each other, nor over dy, x, pre or h")
         new = torch.zeros if T == 0 else torch.empty
         given = {k: t is not None for k, t in (("dw1", dw1), ("db1", db1), ("dw2", dw2), ("db2", db2))}

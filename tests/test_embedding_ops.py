@@ -228,3 +228,40 @@ def test_gradient_over_its_input_is_refused(device):
     d = torch.ones(4, 8, dtype=torch.bfloat16, device=device)
     with pytest.raises(ValueError):
         ops.embedding_bwd(ids, d, 4, out=d)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_gradient_partly_over_its_input_is_refused(device):
+    ids = torch.tensor([0, 1, 0, 3, 2, 2], device=device)
+    buf = torch.ones(12, 8, dtype=torch.bfloat16, device=device)
+    for out, dout in ((buf[:4], buf[3:9]), (buf[5:9], buf[:6]), (buf[:8], buf[1:7])):
+        with pytest.raises(ValueError):
+            ops.embedding_bwd(ids, dout, out.shape[0], out=out)
+    want = ops.embedding_bwd(ids, buf[6:], 4)
+    assert torch.equal(ops.embedding_bwd(ids, buf[6:], 4, out=buf[2:6]), want)
+
+
+def test_shared_memory_against_a_count_of_who_touches_what():
+    import random
+
+    from mxtrain.ops import _lib
+    rng, buf = random.Random(1), torch.zeros(400)
+
+    def view():
+        if rng.random() < 0.2:
+            return buf[rng.randint(0, 200):][:rng.randint(1, 60)]
+        ld = rng.choice((0, 8, 16, 24))
+        return torch.as_strided(buf, (rng.randint(1, 6), rng.randint(1, max(ld, 8))), (ld, 1), rng.randint(0, 200))
+
+    def cells(t):
+        at = torch.zeros(400)
+        torch.as_strided(at, t.shape, t.stride(), t.storage_offset()).fill_(1)
+        return at
+    refused = shared = 0
+    for _ in range(2000):
+        a, b = view(), view()
+        both = bool((cells(a) * cells(b)).any())
+        got = _lib.lies_over((a,), (b,))
+        assert got == _lib.lies_over((a, b), ()) and got == _lib.lies_over((b,), (a,)) and (got or not both)
+        refused, shared = refused + got, shared + both
+    assert refused < 1.1 * shared + 50          # (ranges that only interleave are refused too)

@@ -371,3 +371,34 @@ def test_a_plan_is_returned_though_another_thread_clears_the_table(monkeypatch):
     for kept in ({}, dict(gated._PLANS)):
         monkeypatch.setattr(gated, "_PLANS", Cleared(kept))
         assert (gated._plan_pair(1003, 768, 2048, 768), gated._plan("gate", 1003, 4096, 768)) == first
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_gradient_buffers_partly_over_operands_are_refused(device):
+    """By one row or one value as much as from their start; side by side in one buffer they are taken."""
+    T, H, F = 24, 16, 8
+    x, w1, b1, w2, b2, dy = _make(T, H, F, H, True, device=device)
+    y, pre, h = ops.gated_mlp_fwd(x, w1, b1, w2, b2)
+    e = lambda *s: torch.zeros(*s, dtype=x.dtype, device=device)
+
+    def bwd(x=x, dy=dy, pre=pre, h=h, **kw):
+        return ops.gated_mlp_bwd(dy, x, pre, h, w1, b1, w2, b2, **kw)
+    want = bwd()
+    both = e(T + 15, H)                                    # x: rows 15 .. 38; dw1: rows 0 .. 15
+    both[15:] = x
+    mixed = e(2 * F * H + H * F)
+    flat = e(T * 2 * F + 2 * F)
+    flat[8:8 + T * 2 * F] = pre.reshape(-1)
+    for call in (lambda: bwd(x=both[15:], dw1=both[:2 * F]),
+                 lambda: bwd(pre=flat[8:8 + T * 2 * F].view(T, 2 * F), db1=flat[:2 * F]),
+                 lambda: bwd(pre=flat[8:8 + T * 2 * F].view(T, 2 * F), db2=flat[T * 2 * F:T * 2 * F + H]),
+                 lambda: bwd(dw1=mixed[:2 * F * H].view(2 * F, H), dw2=mixed[2 * F * H - 8:-8].view(H, F)),
+                 lambda: bwd(dw2=mixed[8:8 + H * F].view(H, F), db2=mixed[H * F:H * F + H])):
+        with pytest.raises(ValueError):
+            call()
+    wide = e(T, 2 * H + 8)                                 # columns of one buffer: x, and behind it dw1
+    wide[:, :H] = x
+    apart = bwd(x=wide[:, :H], dw1=wide[:2 * F, H:2 * H], dw2=mixed[:H * F].view(H, F), db1=mixed[H * F:H * F + 2 * F])
+    for a, b in zip(apart, want):
+        assert torch.equal(a, b)
+    assert torch.equal(wide[:, :H], x)
