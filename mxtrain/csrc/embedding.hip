@@ -27,28 +27,28 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const int64_t* __res
                                                             float scale, const int64_t* __restrict__ pos,
                                                             const uint16_t* __restrict__ wpe, int P,
                                                             uint16_t* __restrict__ out, int T, int H) {
-  const int t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
-  if (t >= T) return;
-  const int64_t id = ids[t] - vstart;
-  const bool in = id >= 0 && id < V;                 // (another vocabulary shard's token: zero)
-  const uint16_t* row = wte + (in ? id : 0) * (int64_t)H;
-  const int64_t p = pos ? pos[t] : -1;
-  const uint16_t* prow = p >= 0 && p < P ? wpe + p * (int64_t)H : nullptr;
-  uint16_t* orow = out + (int64_t)t * H;
+  for (int t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); t < T; t += gridDim.x * 4) {
+    const int64_t id = ids[t] - vstart;
+    const bool in = id >= 0 && id < V;                 // (another vocabulary shard's token: zero)
+    const uint16_t* row = wte + (in ? id : 0) * (int64_t)H;
+    const int64_t p = pos ? pos[t] : -1;
+    const uint16_t* prow = p >= 0 && p < P ? wpe + p * (int64_t)H : nullptr;
+    uint16_t* orow = out + (int64_t)t * H;
 #pragma unroll 4
-  for (int c = lane * 8; c < H; c += 512) {
-    float f[8];
-    unpack8(*reinterpret_cast<const uint4*>(row + c), f);
+    for (int c = lane * 8; c < H; c += 512) {
+      float f[8];
+      unpack8(*reinterpret_cast<const uint4*>(row + c), f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = in ? f[j] * scale : 0.f;
-    if (prow) {
-      float g[8];
-      unpack8(*reinterpret_cast<const uint4*>(prow + c), g);
+      for (int j = 0; j < 8; ++j) f[j] = in ? f[j] * scale : 0.f;
+      if (prow) {
+        float g[8];
+        unpack8(*reinterpret_cast<const uint4*>(prow + c), g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] += g[j];
+        for (int j = 0; j < 8; ++j) f[j] += g[j];
+      }
+      *reinterpret_cast<uint4*>(orow + c) = pack8(f);
     }
-    *reinterpret_cast<uint4*>(orow + c) = pack8(f);
   }
 }
 
@@ -340,10 +340,11 @@ SortPlan sort_plan(int T, int V) {
 
 MX_EXPORT int mx_embedding_fwd(const void* ids, const void* wte, int64_t vstart, int V, float scale, const void* pos,
                                const void* wpe, int P, void* out, int T, int H, hipStream_t s) {
-  if (!ids || !wte || !out || T <= 0 || V <= 0 || H <= 0 || (H & 7) || (pos && (!wpe || P <= 0)))
+  if (!ids || !wte || !out || T <= 0 || T > (1 << 30) || V <= 0 || H <= 0 || (H & 7) || (pos && (!wpe || P <= 0)))
     return hipErrorInvalidValue;
   if (((uintptr_t)wte | (uintptr_t)wpe | (uintptr_t)out) & 15) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(embedding_fwd_kernel, dim3((T + 3) / 4), dim3(256), 0, s, (const int64_t*)ids,
+  // (a launch has fewer than 2^32 threads: beyond 2^25 tokens a wave takes several)
+  hipLaunchKernelGGL(embedding_fwd_kernel, dim3(T > 1 << 25 ? 1 << 23 : (T + 3) / 4), dim3(256), 0, s, (const int64_t*)ids,
                      (const uint16_t*)wte, vstart, V, scale, (const int64_t*)pos, (const uint16_t*)wpe, P,
                      (uint16_t*)out, T, H);
   return hipGetLastError();

@@ -14,6 +14,8 @@ import torch
 
 from . import _lib
 
+MAX_COUNT = 1 << 30     # tokens, rows and columns (the kernels count them in 32 bits)
+
 
 def _acc(t):   # at least float32
     return t.double() if t.dtype == torch.float64 else t.float()
@@ -82,6 +84,9 @@ def embedding_fwd(ids, wte, scale: float = 1.0, positions=None, wpe=None, vocab_
             loc, ok = _local(positions, 0, wpe.shape[0])
             out = out + torch.where(ok[:, None], _acc(wpe)[loc.clamp(0, wpe.shape[0] - 1)], zero)
         return out.to(wte.dtype)
+    if max(T, V, H) > MAX_COUNT or (wpe is not None and wpe.shape[0] > MAX_COUNT):
+        raise ValueError(f"{name}: the GPU kernels take at most 2^30 tokens, rows and columns, got {T}, {V} "
+                         f"(positions: {0 if wpe is None else wpe.shape[0]}), {H}")
     _check_hip(name, "wte", wte, H)
     if wpe is not None:
         _check_hip(name, "wpe", wpe, H)

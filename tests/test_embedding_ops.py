@@ -265,3 +265,30 @@ def test_shared_memory_against_a_count_of_who_touches_what():
         assert got == _lib.lies_over((a, b), ()) and got == _lib.lies_over((b,), (a,)) and (got or not both)
         refused, shared = refused + got, shared + both
     assert refused < 1.1 * shared + 50          # (ranges that only interleave are refused too)
+
+
+def test_sizes_that_the_kernels_do_not_count_are_refused(monkeypatch):
+    """Counts go through 32 bits: one that does not fit is named, not cut.  (No memory behind these tensors.)"""
+    from mxtrain.ops import _lib
+    monkeypatch.setattr(_lib, "use_hip", lambda t: True)
+    e = lambda *s, dtype=torch.bfloat16: torch.empty(*s, dtype=dtype, device="meta")
+    ids = lambda n: e(n, dtype=torch.int64)
+    for call in (lambda: ops.embedding_fwd(ids((1 << 30) + 1), e(4, 8)),
+                 lambda: ops.embedding_fwd(ids((1 << 32) + 4), e(4, 8)),
+                 lambda: ops.embedding_fwd(ids(4), e((1 << 32) + 4, 8)),
+                 lambda: ops.embedding_fwd(ids(4), e(4, 8), 1.0, ids(4), e((1 << 32) + 4, 8)),
+                 lambda: ops.embedding_fwd(ids(4), e(4, (1 << 32) + 8))):
+        with pytest.raises(ValueError, match="at most"):
+            call()
+
+
+@gpu
+def test_gpu_lookup_of_more_tokens_than_threads_of_a_launch():
+    """A wave a token: 2^26 tokens are 2^32 threads, more than one launch has."""
+    T, V, H = (1 << 26) + 5, 1000, 8
+    ids = torch.arange(T, device=DEV) * 7 % (V + 3)
+    wte = torch.randn(V, H, device=DEV).to(torch.bfloat16)
+    out = ops.embedding_fwd(ids, wte, 2.0)
+    want = torch.cat([wte * 2.0, torch.zeros(3, H, dtype=torch.bfloat16, device=DEV)])
+    for a, b in zip(out.split(1 << 23), ids.split(1 << 23)):
+        assert torch.equal(a, want[b])

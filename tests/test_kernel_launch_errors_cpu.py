@@ -127,3 +127,10 @@ def test_gated_forward(fake, T):
 def test_gated_input_gradient(fake):
     ok, *failed = _launches(fake, "mx_gated_dx", A, A, 768, A, 1003, 768, 4096, 2, 4, A, None)
     assert ok[:2] == (0, 2) and [r[:2] for r in failed] == [(719, 1), (719, 2)]
+
+
+@pytest.mark.parametrize("T", [1, 1000, (1 << 26) - 3, 1 << 26, 1 << 30])
+def test_threads_of_a_lookup(fake, T):
+    """A launch has fewer than 2^32 threads."""
+    (ok, *_) = _launches(fake, "mx_embedding_fwd", A, A, 0, 1000, 1.0, None, None, 0, A, T, 8, None)
+    assert ok[:2] == (0, 1) and 64 * min(T, 1 << 25) <= ok[2] < 1 << 32
