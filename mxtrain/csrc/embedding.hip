@@ -350,11 +350,14 @@ MX_EXPORT int mx_embedding_fwd(const void* ids, const void* wte, int64_t vstart,
   return hipGetLastError();
 }
 
-// int32 words of workspace: two (key, token) arrays, the block histograms, fp32 partials (16-B aligned)
+// int32 words of workspace: two (key, token) arrays, the block histograms, fp32 partials (16-B aligned); -1: sizes
+// that the kernels do not take
 MX_EXPORT int64_t mx_embedding_bwd_words(int T, int V, int H) {
   if (T <= 0 || V <= 0 || H <= 0 || T > (1 << 30) || V >= (1 << 30)) return -1;
   const SortPlan p = sort_plan(T, V);
   const int64_t t4 = ((int64_t)T + 3) & ~3ll, chunks = (T + CH - 1) / CH;
+  // threads of the sums' launch
+  if (256 * ((chunks * ((H + 511ll) / 512) + 3) / 4 + (V + 63) / 64) >= (int64_t)1 << 32) return -1;
   return 4 * t4 + (((int64_t)p.blocks << p.bits) + 3 & ~3ll) + chunks * 2 * H;
 }
 
@@ -396,7 +399,6 @@ MX_EXPORT int mx_embedding_bwd(const void* ids, int64_t vstart, const void* dout
             (T + CH - 1) / CH, scale, accumulate};
   const int64_t items = (int64_t)u.chunks * u.ncol, sum_blocks = (items + 3) / 4;
   const int64_t zero_blocks = accumulate ? 0 : (V + 63) / 64;
-  if (items >= ((int64_t)1 << 31) || sum_blocks + zero_blocks >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(embedding_sum_kernel, dim3((unsigned)(sum_blocks + zero_blocks)), dim3(256), 0, s, u,
                      (int)sum_blocks);
   if ((e = hipGetLastError()) != hipSuccess || u.chunks == 1) return e;

@@ -134,15 +134,16 @@ def embedding_bwd(keys, dout, rows: int, scale: float = 1.0, out=None, accumulat
         loc, ok = _local(keys, vocab_start, rows)
         acc = torch.zeros(rows, H, dtype=_acc(dout).dtype, device=dev).index_add_(0, loc[ok], _acc(dout)[ok]) * scale
         return out.copy_(_acc(out) + acc if accumulate else acc)
-    if dout.stride(1) != 1 or (T > 1 and (dout.stride(0) < H or dout.stride(0) % 8)) or dout.data_ptr() % 16:
+    words = _lib.query64("mx_embedding_bwd_words", T, rows, H) if max(T, H) <= MAX_COUNT else -1
+    if words < 0:
+        raise ValueError(f"{name}: {T} tokens of {H} columns, {rows} rows are more than the kernels take")
+    if dout.stride(1) != 1 or (T > 1 and (not H <= dout.stride(0) <= MAX_COUNT or dout.stride(0) % 8)) \
+            or dout.data_ptr() % 16:
         dout = dout.clone(memory_format=torch.contiguous_format)
     _check_hip(name, "dout", dout[:1], H)
     keys = keys.contiguous()
     ld = dout.stride(0) if T > 1 else H
     with _lib.on_device(dout):
-        words = _lib.query64("mx_embedding_bwd_words", T, rows, H)
-        if words < 0:
-            raise ValueError(f"{name}: {T} tokens, {rows} rows are more than the kernels take (2^30)")
         ws = torch.empty(words, dtype=torch.int32, device=dev)
         _lib.call("mx_embedding_bwd", _lib.ptr(keys), vocab_start, _lib.ptr(dout), ld, _lib.ptr(out), T, rows, H,
                   scale, int(accumulate), _lib.ptr(ws), words, _lib.stream())

@@ -292,3 +292,26 @@ def test_gpu_lookup_of_more_tokens_than_threads_of_a_launch():
     want = torch.cat([wte * 2.0, torch.zeros(3, H, dtype=torch.bfloat16, device=DEV)])
     for a, b in zip(out.split(1 << 23), ids.split(1 << 23)):
         assert torch.equal(a, want[b])
+
+
+def test_gradient_sizes_that_the_kernels_do_not_count_are_refused(monkeypatch):
+    from mxtrain.ops import _lib
+    monkeypatch.setattr(_lib, "use_hip", lambda t: True)
+    e = lambda *s, dtype=torch.bfloat16: torch.empty(*s, dtype=dtype, device="meta")
+    ids = lambda n: e(n, dtype=torch.int64)
+    for T, H, rows in (((1 << 30) + 1, 8, 4), ((1 << 32) + 4, 8, 4), (4, (1 << 32) + 8, 4),
+                       (1 << 30, 8, (1 << 30) - 1)):      # (together more threads than a launch has)
+        with pytest.raises(ValueError, match="more than the kernels take"):
+            ops.embedding_bwd(ids(T), e(T, H), rows)
+
+
+@gpu
+def test_gpu_gradient_of_rows_far_apart():
+    """A row stride beyond 32 bits (two rows of a buffer of 8 GiB)."""
+    H, ld = 8, (1 << 32) + 8
+    buf = torch.empty(ld + H, dtype=torch.bfloat16, device=DEV)
+    dout = torch.as_strided(buf, (2, H), (ld, 1))
+    dout.copy_(torch.tensor([[1.0], [2.0]]).expand(2, H))
+    buf[H:2 * H] = 7.0
+    got = ops.embedding_bwd(torch.tensor([3, 3], device=DEV), dout, 4)
+    assert (got[:3] == 0).all() and (got[3] == 3.0).all()

@@ -134,3 +134,14 @@ def test_threads_of_a_lookup(fake, T):
     """A launch has fewer than 2^32 threads."""
     (ok, *_) = _launches(fake, "mx_embedding_fwd", A, A, 0, 1000, 1.0, None, None, 0, A, T, 8, None)
     assert ok[:2] == (0, 1) and 64 * min(T, 1 << 25) <= ok[2] < 1 << 32
+
+
+@pytest.mark.parametrize("T,V,H", [(1 << 20, 1 << 29, 8), (1 << 29, 1 << 29, 512), (1 << 30, 1000, 8), (1 << 30, 1 << 29, 8),
+                                   (1 << 30, (1 << 30) - 1, 8), (1 << 30, 1000, 1024)])
+def test_threads_of_an_embedding_gradient(fake, T, V, H):
+    words = _lib.query64("mx_embedding_bwd_words", T, V, H)
+    (ok, *_) = _launches(fake, "mx_embedding_bwd", A, 0, A, H, A, T, V, H, 1.0, 0, A, words, None)
+    if words < 0:
+        assert ok[:2] == (1, 0)
+    else:
+        assert ok[0] == 0 and ok[2] < 1 << 32
