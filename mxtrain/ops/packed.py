@@ -53,6 +53,8 @@ def pack_sequences(cu_seqlens: torch.Tensor, total: int, device=None) -> PackedS
         raise TypeError(f"pack_sequences: cu_seqlens must be int32 or int64, got {cu_seqlens.dtype}")
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
         raise ValueError("pack_sequences: cu_seqlens must be a 1-D tensor of at least two entries")
+    if cu_seqlens.numel() > 1 << 30:      # (counted in 32 bits)
+        raise ValueError(f"pack_sequences: at most 2^30 entries of cu_seqlens, got {cu_seqlens.numel()}")
     total = int(total)
     if not 0 < total <= 1 << 30:
         raise ValueError(f"pack_sequences: total must be in 1 .. 2^30, got {total}")

@@ -131,3 +131,9 @@ def test_no_split_of_a_key_block_is_empty(heads, D, kb):
                 assert (nsp - 1) * per < items, (T, n, items, nsp)
                 split.add(nsp)
     assert split
+
+
+def test_more_sequences_than_the_table_counts_are_refused():
+    for n in ((1 << 30) + 2, (1 << 32) + 3):
+        with pytest.raises(ValueError, match="2\\^30"):
+            ops.pack_sequences(torch.empty(n, dtype=torch.int64, device="meta"), 8)
