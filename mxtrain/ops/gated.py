@@ -263,12 +263,13 @@ def gated_mlp_bwd(dy, x, pre, h, w1, b1, w2, b2, act: str = "silu", dw1=None, db
         ya, da = _act(act, a)
         dh = _acc(dy) @ _acc(w2)
         dpre = torch.cat([dh * b * da, dh * ya], 1)
+        dx = (dpre @ _acc(w1)).to(x.dtype) if need_dx else None     # (before a gradient is written over w1)
         if need_dw:
             for buf, val in ((dw1, dpre.t() @ _acc(x)), (db1, dpre.sum(0)), (dw2, _acc(dy).t() @ _acc(h)),
                              (db2, _acc(dy).sum(0))):
                 if buf is not None:
                     buf.copy_(_acc(buf) + val if accumulate else val)
-        return ((dpre @ _acc(w1)).to(x.dtype) if need_dx else None), dw1, db1, dw2, db2
+        return dx, dw1, db1, dw2, db2
     with _lib.on_device(x):
         s = _lib.stream()
         dpre = torch.empty(T, 2 * F, dtype=x.dtype, device=x.device)

@@ -402,3 +402,14 @@ def test_gradient_buffers_partly_over_operands_are_refused(device):
     for a, b in zip(apart, want):
         assert torch.equal(a, b)
     assert torch.equal(wide[:, :H], x)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_gradients_in_place_of_the_weights(device):
+    """The weights are read before their gradients are written."""
+    x, w1, b1, w2, b2, dy = _make(40, 16, 24, 8, True, device=device)
+    y, pre, h = ops.gated_mlp_fwd(x, w1, b1, w2, b2)
+    want = ops.gated_mlp_bwd(dy, x, pre, h, w1, b1, w2, b2)
+    a, c = w1.clone(), w2.clone()
+    for p, q in zip(ops.gated_mlp_bwd(dy, x, pre, h, a, b1, c, b2, dw1=a, dw2=c), want):
+        assert torch.equal(p, q)
