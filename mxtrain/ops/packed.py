@@ -8,7 +8,7 @@ batch, shared by every layer and by forward and backward.  Tensors are token-maj
 
 Rows behind the last sequence (a batch padded to a fixed size, so a captured step keeps its
 shapes) never matter, whatever they hold: in tensors the op allocates they are zero, in buffers the
-caller passes they are left as they were.
+caller passes they are left as they were.  A value that is not finite reaches only the rows that see it.
 
 On the GPU scores, softmax statistics and sums are fp32; P and dS are rounded once to bf16 as operands of
 the matrix products, and delta = do . o is taken from the bf16 ``o`` that forward returned.
@@ -156,7 +156,25 @@ def _acc(t):   # at least float32
     return t.double() if t.dtype == torch.float64 else t.float()
 
 
-def _ref_fwd(q, k, v, seqs, Hq, Hkv, D, scale):
+def _ref_parts(seqs, *mats):
+    """(rows, keys) ranges that are taken by themselves so that a value that is not finite reaches only the
+    rows that see it (0 * NaN is NaN inside a product): each row of a sequence that holds one, any other
+    sequence whole; None: everything is finite."""
+    nv = int(seqs.meta[0])
+    bad = torch.zeros(nv, dtype=torch.bool, device=seqs.device)
+    for t in mats:
+        bad |= ~torch.isfinite(t.detach()[:nv]).all(1)
+    if not bad.any():
+        return None
+    parts, a, ends = [], 0, seqs.end.tolist()
+    while a < nv:
+        b = ends[a]
+        parts += [((i, i + 1), (a, i + 1)) for i in range(a, b)] if bad[a:b].any() else [((a, b), (a, b))]
+        a = b
+    return parts
+
+
+def _ref_fwd(q, k, v, seqs, Hq, Hkv, D, scale, dout=None):
     T = seqs.total
     real = torch.arange(T, device=q.device) < seqs.meta[0]
 
@@ -164,11 +182,21 @@ def _ref_fwd(q, k, v, seqs, Hq, Hkv, D, scale):
         return torch.where(real[:, None], _acc(t), torch.zeros((), dtype=_acc(t).dtype)).reshape(T, h, D).transpose(0, 1)
     g = Hq // Hkv
     qf, kf, vf = heads(q, Hq), heads(k, Hkv).repeat_interleave(g, 0), heads(v, Hkv).repeat_interleave(g, 0)
-    m = _ref_mask(seqs)
-    s = (torch.matmul(qf, kf.transpose(1, 2)) * scale).masked_fill(~m, float("-inf"))
-    lse = torch.logsumexp(s, -1)
-    p = torch.where(m, torch.exp(s - lse[..., None]), torch.zeros((), dtype=s.dtype))
-    o = torch.matmul(p, vf).transpose(0, 1).reshape(T, Hq * D)
+
+    def attend(qf, kf, vf, m):
+        s = (torch.matmul(qf, kf.transpose(1, 2)) * scale).masked_fill(~m, float("-inf"))
+        lse = torch.logsumexp(s, -1)
+        p = torch.where(m, torch.exp(s - lse[..., None]), torch.zeros((), dtype=s.dtype))
+        return torch.matmul(p, vf), lse
+    m, parts = _ref_mask(seqs), _ref_parts(seqs, q, k, v, *(() if dout is None else (dout,)))
+    if parts is None:
+        o, lse = attend(qf, kf, vf, m)
+    else:
+        got = [attend(qf[:, a:b], kf[:, c:d], vf[:, c:d], m[a:b, c:d]) for (a, b), (c, d) in parts]
+        rest = T - parts[-1][0][1]
+        o = torch.cat([x for x, _ in got] + [qf.new_zeros(Hq, rest, D)], 1)
+        lse = torch.cat([x for _, x in got] + [qf.new_zeros(Hq, rest)], 1)
+    o = o.transpose(0, 1).reshape(T, Hq * D)
     lse = torch.where(real, lse * LOG2E, torch.full_like(lse, float("inf")))
     return o, lse
 
@@ -232,7 +260,7 @@ def packed_attn_bwd(dout, q, k, v, o, lse, seqs: PackedSequences, Hq: int, Hkv: 
     if m is None:
         with torch.enable_grad():
             leaves = [_acc(t.detach()).clone().requires_grad_(True) for t in (q, k, v)]
-            of, _ = _ref_fwd(*leaves, seqs, Hq, Hkv, D, scale)
+            of, _ = _ref_fwd(*leaves, seqs, Hq, Hkv, D, scale, dout)
             nv = int(seqs.meta[0])
             grads = torch.autograd.grad(of[:nv], leaves, _acc(dout)[:nv])
         return tuple(_emit(g.to(q.dtype), buf, seqs) for g, buf in zip(grads, (dq, dk, dv)))

@@ -137,3 +137,52 @@ def test_more_sequences_than_the_table_counts_are_refused():
     for n in ((1 << 30) + 2, (1 << 32) + 3):
         with pytest.raises(ValueError, match="2\\^30"):
             ops.pack_sequences(torch.empty(n, dtype=torch.int64, device="meta"), 8)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_non_finite_values_reach_only_the_rows_that_see_them(bad):
+    torch.manual_seed(3)
+    lens, pad, Hq, Hkv, D = [7, 1, 9, 6], 3, 4, 2, 8
+    T = sum(lens) + pad
+    s = ops.pack_sequences(_cu(lens), T)
+    q, k, v, do = (torch.randn(T, h * D, dtype=torch.float64) for h in (Hq, Hkv, Hkv, Hq))
+    want = attention(q, k, v, lens, Hq, Hkv, D, D ** -0.5, do)
+
+    def go(at, *which):
+        x = [t.clone() for t in (q, k, v, do)]
+        for i in which:
+            x[i][at] = bad
+        o, lse = ops.packed_attn_fwd(*x[:3], s, Hq, Hkv, D)
+        return dict(zip(("o", "lse", "dq", "dk", "dv"),
+                        (o, lse, *ops.packed_attn_bwd(x[3], *x[:3], o, lse, s, Hq, Hkv, D))))
+
+    def same(t, name, rows):
+        ref = want[name][0]
+        if name == "lse":
+            t, ref = t.double().t(), ref.float().double().t()
+        torch.testing.assert_close(t[rows], ref[rows], rtol=1e-6 if name == "lse" else 1e-12, atol=1e-12)
+    got = go([3, 20, 24, 25], 0, 1, 2, 3)         # in the first and the last sequence and behind them
+    for name in got:
+        same(got[name], name, slice(7, 17))
+    same(got["o"], "o", slice(0, 3))              # (rows before the bad ones)
+    same(got["dq"], "dq", slice(0, 3))
+    for name in ("dk", "dv"):
+        assert torch.isnan(got[name][:7]).all()   # (every key is seen by a row that sees the bad ones)
+        assert (got[name][23:] == 0).all()
+    assert torch.isnan(got["o"][3:7]).all() and (got["o"][23:] == 0).all()
+    got = go([12], 3)                             # a row of dout: its own dq, and dk, dv of the keys it sees
+    for name, rows in (("dq", 12), ("dk", slice(8, 13)), ("dv", slice(8, 13))):
+        assert not torch.isfinite(got[name][rows]).any()
+    for name, rows in (("dq", slice(13, 17)), ("dq", slice(8, 12)), ("dk", slice(13, 17)), ("dv", slice(13, 17))):
+        same(got[name], name, rows)
+
+
+def test_large_finite_values_of_masked_pairs_on_the_cpu():
+    torch.manual_seed(4)
+    s, T = ops.pack_sequences(_cu([5, 6]), 11), 11
+    q, k, v, do = (torch.randn(T, 8) for _ in range(4))
+    do[:5] *= 1e20
+    v[5:] *= 1e20
+    o, lse = ops.packed_attn_fwd(q, k, v, s, 1, 1, 8)
+    for name, t in zip(("dq", "dk", "dv"), ops.packed_attn_bwd(do, q, k, v, o, lse, s, 1, 1, 8)):
+        within(t, attention(q, k, v, [5, 6], 1, 1, 8, 8 ** -0.5, do)[name], name)
