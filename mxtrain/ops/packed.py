@@ -271,7 +271,8 @@ def packed_attn_bwd(dout, q, k, v, o, lse, seqs: PackedSequences, Hq: int, Hkv: 
     if given:
         wide, narrow = Hq * D, Hkv * D
         _apart("packed_attn_bwd", T, [(*g, w) for g, w in zip(grads, (wide, narrow, narrow))],
-               [(q_, ldq, wide), (k_, ldk, narrow), (v_, ldv, narrow), (o_, ldo, wide), (do_, lddo, wide)])
+               [(q_, ldq, wide), (k_, ldk, narrow), (v_, ldv, narrow), (o_, ldo, wide), (do_, lddo, wide),
+                (lse.data_ptr(), 2 * Hq, 2 * Hq)])     # (lse: as many bytes as [T, 2 Hq] of bf16)
     with _lib.on_device(q):
         if not given:
             dq = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device)

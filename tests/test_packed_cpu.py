@@ -186,3 +186,15 @@ def test_large_finite_values_of_masked_pairs_on_the_cpu():
     o, lse = ops.packed_attn_fwd(q, k, v, s, 1, 1, 8)
     for name, t in zip(("dq", "dk", "dv"), ops.packed_attn_bwd(do, q, k, v, o, lse, s, 1, 1, 8)):
         within(t, attention(q, k, v, [5, 6], 1, 1, 8, 8 ** -0.5, do)[name], name)
+
+
+def test_gradients_over_the_statistics_are_refused(monkeypatch):
+    from mxtrain.ops import _lib
+    T, H, D = 8, 2, 64
+    s = ops.pack_sequences(_cu([5, 3]), T)
+    q, k, v, do, o, dk, dv = (torch.randn(T, H * D).bfloat16() for _ in range(7))
+    mem = torch.zeros(T * H * D, dtype=torch.bfloat16)
+    lse = mem.view(torch.float32)[-H * T:].view(H, T)
+    monkeypatch.setattr(_lib, "use_hip", lambda t: True)
+    with pytest.raises(ValueError, match="must not lie over"):
+        ops.packed_attn_bwd(do, q, k, v, o, lse, s, H, H, D, dq=mem.view(T, H * D), dk=dk, dv=dv)
