@@ -315,3 +315,56 @@ def test_gpu_gradient_of_rows_far_apart():
     buf[H:2 * H] = 7.0
     got = ops.embedding_bwd(torch.tensor([3, 3], device=DEV), dout, 4)
     assert (got[:3] == 0).all() and (got[3] == 3.0).all()
+
+
+def _in_order(keys, dout, rows, scale, order):
+    """The gradient's fp32 sums, addition by addition: tokens in ``order`` (by key), 32 of them at a time,
+    then the sums of a key that runs over several in order; one rounding at the end."""
+    keys, d = keys[order].tolist(), dout.float()[order]
+    table = torch.zeros(rows, dout.shape[1])
+    t = 0
+    while t < len(keys):
+        end = t
+        while end < len(keys) and keys[end] == keys[t]:
+            end += 1
+        total, e = None, t
+        while e < end:
+            stop = min(end, (e // 32 + 1) * 32)
+            acc = torch.zeros(dout.shape[1])
+            for i in range(e, stop):
+                acc = acc + d[i]
+            total, e = acc if total is None else total + acc, stop
+        if 0 <= keys[t] < rows:
+            table[keys[t]] = total * scale
+        t = end
+    return table.to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("kind", ["any", "one", "rank"])
+@pytest.mark.parametrize("T,V", [(100, 7), (8192, 900), (8193, 900), (9000, 40)])
+@pytest.mark.parametrize("device", [pytest.param("cuda", marks=pytest.mark.gpu), "cpu"])
+def test_sums_are_those_of_token_order(device, T, V, kind):
+    """Bit for bit, on values whose fp32 sum depends on the order of its terms: of a key's tokens the first is
+    large, the third takes it away again, the second is lost beside it and the fourth is not, and so on.  (CPU:
+    that it does.)"""
+    gen = torch.Generator().manual_seed(T + V)
+    H = 8
+    keys = _ids(kind, T, V, gen)
+    stable = torch.argsort(keys, stable=True)
+    _, count = torch.unique_consecutive(keys[stable], return_counts=True)
+    turn = torch.cat([torch.arange(int(n)) for n in count]) % 4
+    large = 2.0 ** torch.randint(26, 30, (T, H), generator=gen)
+    large[2:] = torch.where((turn[2:] == 2)[:, None], -large[:-2], large[2:])
+    dout = torch.empty(T, H)
+    pair = torch.zeros(T, dtype=torch.bool)          # (a first without its third stays small)
+    pair[2:] = turn[2:] == 2
+    pair[:-2] |= turn[2:] == 2
+    dout[stable] = torch.where(pair[:, None], large, torch.rand(T, H, generator=gen) + 0.5)
+    dout = dout.to(torch.bfloat16)
+    want = _in_order(keys, dout, V, 0.75, stable)
+    if device == "cpu":
+        back = T - 1 - torch.argsort(keys.flip(0), stable=True)       # equal keys from the last to the first
+        assert torch.equal(keys[back], keys[stable]) and not torch.equal(_in_order(keys, dout, V, 0.75, back), want)
+        return
+    got = ops.embedding_bwd(keys.to(DEV), dout.to(DEV), V, 0.75).cpu()
+    assert torch.equal(got, want)
