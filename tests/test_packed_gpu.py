@@ -420,3 +420,42 @@ def test_large_finite_values_of_masked_pairs(D, heads, lens, inside):
     grads = ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D)
     for name, t in zip(("o", "dq", "dk", "dv"), (o, *grads)):
         within(t, want[name], name)
+
+
+def _mixed(T, longest, seed):
+    gen, out = torch.Generator().manual_seed(seed), []
+    while sum(out) < T:
+        out.append(min(int(torch.randint(1, longest, (1,), generator=gen)), T - sum(out)))
+    return out
+
+
+@pytest.mark.parametrize("T,longest", [(1000, 300), (262144, 900), (262401, 60000), (600001, 3000)])
+def test_dispatch_lists(T, longest):
+    """Every block once (by work up to 2048 blocks), and the query tiles before each 256-key block."""
+    s = ops.pack_sequences(_cu(_mixed(T, longest, T)), T, device=DEV)
+    start, end, order = s.start.cpu().long(), s.end.cpu().long(), s.order.cpu().long()
+    at = 0
+    for which, B in (("query", 128), ("key", 128), ("key", 256)):
+        nb = -(-T // B)
+        first, last = torch.arange(nb) * B, (torch.arange(nb) * B + B).clamp_max(T)
+        work = last - start[first] if which == "query" else end[last - 1] - first
+        mine = order[at:at + nb]
+        assert torch.equal(mine.sort().values, torch.arange(nb))
+        if nb <= 2048:
+            assert (work[mine].diff() <= 0).all()
+        at += nb
+    before = s.order[at + at % 2:].view(torch.int64).cpu()
+    assert torch.equal(before[:nb + 1], torch.cat([torch.zeros(1, dtype=torch.int64), ((work + 63) // 64).cumsum(0)]))
+
+
+@pytest.mark.parametrize("T,heads,D,longest", [(262500, (2, 2), 64, 900), (17000, (8, 4), 128, 2000), (40000, (16, 2), 128, 3000)])
+def test_many_blocks(T, heads, D, longest):
+    """Blocks in sequence order, and shares that begin past the 64th key block of a head."""
+    Hq, Hkv = heads
+    lens = _mixed(T, longest, T)
+    q, k, v, do = _inputs(T, Hq, Hkv, D, seed=71)
+    s = ops.pack_sequences(_cu(lens), T, device=DEV)
+    o, lse = ops.packed_attn_fwd(q, k, v, s, Hq, Hkv, D)
+    want = attention(q, k, v, lens, Hq, Hkv, D, D ** -0.5, do)
+    for name, t in zip(("o", "dq", "dk", "dv"), (o, *ops.packed_attn_bwd(do, q, k, v, o, lse, s, Hq, Hkv, D))):
+        within(t, want[name], name)
