@@ -23,6 +23,7 @@ import torch
 from . import _lib
 
 LOG2E = 1.4426950408889634
+SCALES = 2.0 ** -100, 2.0 ** 100     # of the GPU kernels: lse / (scale log2 e) stays in the fp32 range
 
 
 class PackedSequences:
@@ -95,6 +96,8 @@ def _check(name, seqs, Hq, Hkv, D, scale, **mats):
         raise ValueError(f"{name}: scale must be positive and finite, got {scale}")
     q = mats["q"]
     hip = _lib.use_hip(q)
+    if hip and not SCALES[0] <= scale <= SCALES[1]:
+        raise ValueError(f"{name}: the GPU kernels take a scale of 2^-100 .. 2^100, got {scale}")
     if hip and D not in (64, 128):
         raise ValueError(f"{name}: the GPU kernels take a head dimension of 64 or 128, got {D}")
     for key, t in mats.items():
@@ -132,7 +135,7 @@ def _mats(seqs, Hq, Hkv, D, scale, q, *mats):
     """[(address, row stride)] of a valid GPU call's matrices (None for those not given), or None: a
     CPU call, or one whose fault :func:`_check` names."""
     if (type(seqs) is not PackedSequences or not _lib.use_hip(q) or (D != 64 and D != 128) or Hkv <= 0 or Hq <= 0
-            or Hq % Hkv or not (scale is None or 0.0 < scale < math.inf)):
+            or Hq % Hkv or not (scale is None or SCALES[0] <= scale <= SCALES[1])):
         return None
     dev, T, out = seqs.start.get_device(), seqs.total, []
     for t, heads in mats:

@@ -198,3 +198,18 @@ def test_gradients_over_the_statistics_are_refused(monkeypatch):
     monkeypatch.setattr(_lib, "use_hip", lambda t: True)
     with pytest.raises(ValueError, match="must not lie over"):
         ops.packed_attn_bwd(do, q, k, v, o, lse, s, H, H, D, dq=mem.view(T, H * D), dk=dk, dv=dv)
+
+
+def test_scales_beyond_the_kernels_range_are_refused(monkeypatch):
+    """They hold the scale, and lse divided by it, in fp32."""
+    from mxtrain.ops import _lib
+    T, H, D = 8, 2, 64
+    s = ops.pack_sequences(_cu([5, 3]), T)
+    q = torch.randn(T, H * D).bfloat16()
+    o, lse = ops.packed_attn_fwd(q, q, q, s, H, H, D, 1e-39)          # (taken on the CPU)
+    monkeypatch.setattr(_lib, "use_hip", lambda t: True)
+    for scale in (1e-50, 1e-39, 1e31, 1e300):
+        with pytest.raises(ValueError, match="scale"):
+            ops.packed_attn_fwd(q, q, q, s, H, H, D, scale)
+        with pytest.raises(ValueError, match="scale"):
+            ops.packed_attn_bwd(q, q, q, q, o, lse, s, H, H, D, scale)
