@@ -15,7 +15,7 @@ called by every rank of a job (bench.py, the launcher) BEFORE it initialises its
    staged kernels), the autotune (every op x message size checked bit-exact against RCCL
    and timed) and a p2p round trip with both ring neighbours (the 1F1B channel);
 3. each rank posts its child's exit code / verdict; rank 0 writes ONE verdict that every
-   rank reads.  Any non-zero exit, fault, timeout or failed check on any rank ->
+   rank reads, and waits until all have (the store may end with it).  Any non-zero exit, fault, timeout or failed check on any rank ->
    ``MXTRAIN_XGMI=0`` on every rank (RCCL everywhere), with the reason.
 
 The reference has no such step: its collectives are NCCL over NVSwitch/EFA inside the
@@ -87,6 +87,14 @@ def should_run(world: int, xgmi_mode: str) -> bool:
         return True
     import torch
     return torch.cuda.device_count() > 0   # (counting devices does not initialise the GPU)
+
+
+def _quiet(f, *args):
+    """The verdict is known: what is left can only fail with the rank at the other end."""
+    try:
+        f(*args)
+    except Exception:   # noqa: BLE001
+        pass
 
 
 def run_preflight(world: int, rank: int, timeout_s: float = 150.0) -> Dict:
@@ -168,8 +176,10 @@ def run_preflight(world: int, rank: int, timeout_s: float = 150.0) -> Dict:
                         if k in res[0]:
                             verdict[k] = res[0][k]
             store.set("verdict", json.dumps(verdict))
+            _quiet(store.wait, [f"read/{r}" for r in range(1, world)], timedelta(seconds=60))   # (the store may be ours)
         else:
             verdict = json.loads(store.get("verdict").decode())
+            _quiet(store.set, f"read/{rank}", "1")
     except Exception as e:   # noqa: BLE001 -- the store itself failed: RCCL, reason recorded
         verdict = {"ok": False, "reason": f"preflight error: {e!r}"[:300]}
     verdict["s"] = round(time.time() - t0, 1)
