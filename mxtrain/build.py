@@ -41,7 +41,9 @@ HIP_FLAGS = [
     "-fvisibility=hidden",
     "-ffp-contract=fast",
     "-Wno-unused-result",
-    # no packed fp32 math (v_pk_add / mul / fma_f32): scalar forms only, rounding unchanged
+    # no packed fp32 math (v_pk_add / mul / fma_f32): scalar forms only.  The compiler contracts more of
+    # these to one rounding (LayerNorm forward and backward, query-major flash attention, batch-norm and
+    # column statistics, RoIAlign, IoU, loss and norm reductions): last bits differ from a build without it
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 

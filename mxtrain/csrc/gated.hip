@@ -19,9 +19,12 @@
 // multiple of 8 is taken without padding.  16 x 16 x 32 MFMA with the weight (column) operand
 // first, so that a lane holds 4 consecutive columns of a row.
 //
-// Large products are bound by their K loop: at 128 x 64 a wave the fragment reads from LDS take as long
-// as the matrix pipe (1.1 - 1.25 PFLOP/s; forward and backward of 4096 x 4096 x 10880 in 2.9 ms).  Short
-// ones (4096 x 1024 x 2688: 0.26 ms) by rounds of workgroups that fill and drain for 16 - 84 steps.
+// Large products (4096 x 4096 x 10880, forward and backward in 2.95 ms) run at 0.74 PFLOP/s (gate gradient) to 1.15
+// (dx): gate 765 us, down 325, where library products of these shapes without an epilogue take 618 and 231.
+// At 256 x 256 one workgroup holds a CU, so an epilogue's memory traffic (178 MB in and 178 out for the gate
+// gradient) runs beside no products; and the K-contiguous loop waits for more than its LDS reads, or it would
+// match the library's.  Short ones (4096 x 1024 x 2688: 0.27 ms) are bound by rounds of workgroups that fill and
+// drain for 16 - 84 steps.
 #include "gemm_common.h"
 
 #include <type_traits>

@@ -219,8 +219,11 @@ __device__ __forceinline__ int pair_rank(int rank, int n) {
 // (S^T = K Q^T, O^T = V^T P^T), so the softmax statistics are lane-local plus one half exchange.
 // K / V tiles of BK keys arrive by LDS-DMA into a two-slot ring, one barrier per tile.  Two workgroups a
 // CU, so that one's exponentials run beside the other's products: 16384 tokens in one, 32 heads of 128,
-// forward 2.15 ms (1.03 PFLOP/s), dQ 2.95 (1.12); 4096 of ~300, 16 heads of 64, bound by the latency of a
-// block's few tiles, 20 and 23 us.  HALF: 64 rows, two waves for each 32 (see launch_qmajor).
+// forward 2.15 ms (1.03 PFLOP/s), dQ 2.95 (1.12); 16 heads of 64, 0.72 ms (0.76) and 0.76 (1.08), bound by vector issue (busy
+// 67 and 62 % of the time, the matrix pipe 41 and 53 %: a score costs as many vector operations as with 128
+// columns, for half the products); 4096 of ~300, 16 heads of 64, bound by the latency of a block's few tiles,
+// 20 and 23 us.  The forward of 128 in whole blocks spills 11 registers, which its tile loop reads back.  HALF: 64
+// rows, two waves for each 32 (see launch_qmajor).
 template <int D, bool DQ, bool HALF>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void packed_qmajor_kernel(const PArgs a) {
   constexpr int BQ = HALF ? 64 : 128, BK = D == 64 ? 128 : 64, NSUB = BK / 32, NKK = D / 16, NDT = D / 32;
@@ -573,7 +576,7 @@ constexpr int KB1 = 128, KB2 = 256, QT2 = 64;   // keys of a block (D = 64 / 128
 // Splits of a key block of `items` (query head, query tile) pairs: a split holds a workgroup slot's even
 // share of the batch (meta: the query tiles of all blocks of one head) and a few items more, which pay
 // for its partial sums.  dQ, dK, dV of 8 query heads on one key head, 512 tokens: 73 -> 38 us (D 64),
-// 156 -> 65 us (D 128); without the extra items 4096 tokens of ~300-token documents take 120 us, not 99
+// 156 -> 58 us (D 128); without the extra items 4096 tokens of ~300-token documents take 120 us, not 99
 // (16 heads of 128); with shares twice as large 16384 tokens, 16 / 4 heads, take 4.9 ms, not 3.8.
 // No split is empty (the last would fetch rows and statistics behind the last query head): 88 items in 16
 // splits of 6 are 15.
@@ -712,7 +715,9 @@ __device__ __forceinline__ void redo_keys(const PArgs& a, const KeyOut<D>& out, 
 // those of long sequences are split along their (query head, query tile) items over up to `nsplit`
 // workgroups, whose fp32 partial sums packed_join_kernel adds in order (or all are cut, see KeyShare).
 //
-// D = 64.  Four waves of 32 keys, two waves per SIMD.
+// D = 64.  Four waves of 32 keys, two waves per SIMD.  16384 tokens in one, 16 heads: 1.22 ms (0.90 PFLOP/s), the
+// matrix pipe busy 45 % of the time, the vector pipe 43: a 32-key wave reads LDS for 1.5 cycles to each of the
+// matrix pipe's.
 template <int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void
 packed_kmajor_kernel(const PArgs a) {
@@ -897,7 +902,7 @@ packed_kmajor_kernel(const PArgs a) {
 // two MFMAs (a 32-key wave needs 1408 LDS cycles per 1024 MFMA cycles of the four SIMDs -- the
 // transposed reads run at half rate --, this one 1408 per 2048), and the accumulators of both groups
 // (256 registers), their K rows and half of V (96; the rest is read again from LDS) and S, dP (64) fit
-// the 512 registers.  A workgroup holds 256 keys.  16384 tokens in one, 32 heads: 4.1 ms, 1.07 PFLOP/s,
+// the 512 registers.  A workgroup holds 256 keys.  16384 tokens in one, 32 heads: 4.2 ms, 1.05 PFLOP/s,
 // the matrix pipe busy 45 % of the time: no other wave runs beside a wave's own vector work.
 //
 // MFMA with its accumulator in ordinary registers.  The compiler gives every MFMA of a kernel that
@@ -1274,9 +1279,10 @@ int key_splits(int T, int Hq, int Hkv, int D) {
 }
 // Most shares, one per CU, or 0: shared heads of D = 128 have few key blocks, and shares beat splits
 // once there is work enough to pay for the joining, unless there are blocks enough to keep the CUs
-// evenly busy.  dQ, dK, dV in us by shares and by splits: 8001 tokens of ~900-token documents, 32 / 8
-// heads, 410 and 465; 16384 of ~1000, 8 / 1 heads, 295 and 412; 4096 in one, 16 / 4 heads, 320 and 390;
-// but 4096 of ~300, 8 / 1 heads, 121 and 90; 512 in one 106 and 62; own heads, 8001 of ~900, 270 and 240.
+// evenly busy.  dQ, dK, dV in us by shares and by splits (means of three batches): 8001 tokens of ~900-token
+// documents, 32 / 8 heads, 558 and 624; 16384 of ~1000, 8 / 1 heads, 381 and 547; 4096 in one, 16 / 4 heads, 319 and
+// 391; 4096 of ~300, 16 / 4 heads, 150 and 162; but 4096 of ~300, 8 / 1 heads, 129 and 104; 512 in one 78 and 58; own
+// heads, 8001 of ~900, 326 and 309.
 int key_shares(int T, int Hq, int Hkv, int D) {
   const int64_t blocks = (int64_t)((T + KB2 - 1) / KB2) * Hkv;
   return D == 128 && Hq > Hkv && blocks < 1024 && (int64_t)T * Hq >= 60000 ? 256 : 0;

@@ -5,6 +5,8 @@ positions restart with each sequence (``ops.pack_sequences(...).positions``), ne
 ``embed_fwd`` / ``embed_bwd`` (ops/fused.py) for fixed [B, S] batches.  An id outside
 [vocab_start, vocab_start + V) (another vocabulary shard's) or a position outside the table adds
 nothing, forward and backward.
+
+On the GPU: bfloat16, rows of a multiple of 8 values, at most 2^30 tokens, rows and columns.
 """
 from __future__ import annotations
 

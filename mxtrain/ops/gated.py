@@ -112,7 +112,9 @@ def _mats(act, x, w1, b1, w2, b2):
 # workgroup alone on its CU; us per round of workgroups (one on every slot of the 256 CUs) beside the
 # steps, more of it where the epilogue reads and writes as much as the gate gradient's, and once.
 # Fitted to one MI355X over 4096 x 4096 x 10880 (steps), 4096 x 1024 x 2688 (rounds) and, the small
-# tile, 1003 x 768 x 2048 and 300 x 512 x 1376.
+# tile, 1003 x 768 x 2048 and 300 x 512 x 1376.  Of 85 picks (five products of three of these and of
+# 14 other shapes of 73 .. 3808 tokens) 71 were the fastest and 76 within 5 % of it; the worst took 17 % longer
+# (453 x 504 x 1960 "down", two splits for four).
 _TILES = ((128, 128, 2, 1.14, 0.97, 5.0, 3.5, 0.0), (256, 256, 1, 1.72, 1.72, 5.0, 30.0, 0.0),
           (128, 128, 1, 0.62, 0.62, 4.0, 4.2, 0.0),
           (256, 128, 1, 0.985, 0.985, 5.0, 7.5, 0.0), (64, 128, 2, 0.57, 0.45, 2.5, 3.6, 6.0))
@@ -140,9 +142,10 @@ def _plan(kind, M, N, K):
     128); few tiles leave CUs idle, so smaller ones with a deeper ring win (1003 x 768 x 2048 "gate":
     12.6 us against 24.9), and a long K is split once the tiles cover less than half of the chip
     (its "dx": 21.2 us in 4 splits, 40 us in one).  Tiles of 64 rows, two workgroups a CU, run one's
-    epilogue beside the other's loop, which the gate gradient gains from most (4096 x 1024 x 2688: 50
-    us, 54 with 128 x 128, 61 with 256 x 256; 700 x 2048 x 5504: 31 and 43), and short batches (700 x
-    2048 x 5504 "gate": 49 and 58)."""
+    epilogue beside the other's loop, which the gate gradient gains from most (4096 x 1024 x 2688: 51
+    us, 55 with 128 x 128, 62 with 256 x 256; 700 x 2048 x 5504: 30 and 42), and short batches (700 x
+    2048 x 5504 "gate": 49 and 58).  Each product by itself, again and again; in a pass of the block they
+    find less in the caches (gate gradient of 4096 x 1024 x 2688: 56)."""
     key = (kind, M, N, K)
     best = _PLANS.get(key)
     if best is None:
@@ -165,8 +168,9 @@ def _plan(kind, M, N, K):
 
 def _plan_pair(T, H, F, Ho):
     """The tile of both weight gradients in one launch, or None where two are faster: together they
-    leave one round of workgroups unfilled, not two (4096 x 1024 x 2688: 64 us, apart 58 + 40; 4096 x
-    4096 x 10880: 911 and 630 + 321; 2048 x 2048 x 5504 fills its rounds: 154 and 97 + 56)."""
+    leave one round of workgroups unfilled, not two (4096 x 1024 x 2688: 65 us, apart 98; 4096 x 4096 x
+    10880: 905 and 977; 2048 x 2048 x 5504 fills its rounds: 155 and 157; as in :func:`_plan`, by
+    themselves: in a pass of the block 72 and 990)."""
     key = ("pair", T, H, F, Ho)
     plan = _PLANS.get(key)      # (one look: another thread may clear the table at any time)
     if plan is None:

@@ -10,7 +10,7 @@ Rows behind the last sequence (a batch padded to a fixed size, so a captured ste
 shapes) never matter, whatever they hold: in tensors the op allocates they are zero, in buffers the
 caller passes they are left as they were.  A value that is not finite reaches only the rows that see it.
 
-On the GPU scores, softmax statistics and sums are fp32; P and dS are rounded once to bf16 as operands of
+On the GPU: bfloat16, head dimensions 64 and 128, a scale of 2^-100 .. 2^100.  Scores, softmax statistics and sums are fp32; P and dS are rounded once to bf16 as operands of
 the matrix products, and delta = do . o is taken from the bf16 ``o`` that forward returned.
 """
 from __future__ import annotations
