@@ -276,14 +276,17 @@ def overlap(T, a, b) -> bool:
 def lies_over(outs, ins) -> bool:
     """Whether one of the tensors ``outs`` shares memory with another of them or with one of ``ins``
     (column ranges of one buffer do not)."""
-    span = []
-    for t in (*outs, *ins):
-        p = t.data_ptr()
-        span.append((p, p + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-                     if t.numel() else p, t))
-    for i, (a0, a1, a) in enumerate(span[:len(outs)]):
-        for b0, b1, b in span[i + 1:]:
-            if a0 < b1 and b0 < a1 and not _columns_apart(a, b):
+    all_, span = (*outs, *ins), []
+    for t in all_:
+        p, n = t.data_ptr(), t.numel()
+        if n and not t.is_contiguous():
+            n = 1 + sum((k - 1) * s for k, s in zip(t.shape, t.stride()))
+        span.append((p, p + n * t.element_size()) if n else (0, 0))
+    for i in range(len(outs)):
+        a0, a1 = span[i]
+        for j in range(i + 1, len(all_)):
+            b0, b1 = span[j]
+            if a0 < b1 and b0 < a1 and not _columns_apart(all_[i], all_[j]):
                 return True
     return False
 
