@@ -22,3 +22,13 @@ def _reset_parallel_state():
         pstate._STATE = None
     except Exception:
         pass
+
+
+@pytest.fixture(scope="session")
+def kernel_library():
+    """Path of the kernel library, for CPU tests of its host side (built if nothing is)."""
+    from mxtrain import build
+    from mxtrain.ops import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        build.build_kernels()
+    return _lib.LIB_PATH

@@ -294,7 +294,7 @@ def test_gpu_lookup_of_more_tokens_than_threads_of_a_launch():
         assert torch.equal(a, want[b])
 
 
-def test_gradient_sizes_that_the_kernels_do_not_count_are_refused(monkeypatch):
+def test_gradient_sizes_that_the_kernels_do_not_count_are_refused(monkeypatch, kernel_library):
     from mxtrain.ops import _lib
     monkeypatch.setattr(_lib, "use_hip", lambda t: True)
     e = lambda *s, dtype=torch.bfloat16: torch.empty(*s, dtype=dtype, device="meta")

@@ -354,7 +354,7 @@ def test_gpu_tile_table_matches_the_kernels():
     assert _lib.query("mx_gated_tile", len(gated._TILES), 0) == -1
 
 
-def test_a_plan_is_returned_though_another_thread_clears_the_table(monkeypatch):
+def test_a_plan_is_returned_though_another_thread_clears_the_table(monkeypatch, kernel_library):
     import mxtrain.ops.gated as gated
     monkeypatch.setattr(gated, "_PLANS", {})
     first = gated._plan_pair(1003, 768, 2048, 768), gated._plan("gate", 1003, 4096, 768)

@@ -11,6 +11,8 @@ import pytest
 
 from mxtrain.ops import _lib
 
+pytestmark = pytest.mark.usefixtures("kernel_library")
+
 FAKE = r"""
 #include <stddef.h>
 #include <string.h>
@@ -73,7 +75,6 @@ def fake(tmp_path_factory):
 
 def _launches(fake, name, *args):
     """[(result, launches, most threads of a launch)] of the call with no launch failing, then with each in turn."""
-    _lib.lib()
     codes = {ctypes.c_void_p: "P", ctypes.c_int: "I", ctypes.c_int64: "L", ctypes.c_float: "F"}
     sig = "".join(codes[t] for t in _lib.SIGNATURES[name])
     out = subprocess.run([sys.executable, str(fake / "run.py"), str(fake / "fake.so"), _lib.LIB_PATH,

@@ -109,7 +109,7 @@ def test_overlap_of_strided_matrices():
 
 @pytest.mark.parametrize("D,kb", [(64, 128), (128, 256)])
 @pytest.mark.parametrize("heads", [(8, 1), (4, 1), (16, 4), (32, 8), (20, 5), (12, 12), (16, 16)])
-def test_no_split_of_a_key_block_is_empty(heads, D, kb):
+def test_no_split_of_a_key_block_is_empty(heads, D, kb, kernel_library):
     """Every split of a key block begins at one of its (query head, query tile) items: one that did not
     would fetch the rows and statistics of a query head that is not there.  (Lengths of one document, and
     the first of two, up to where blocks are no longer split.)"""
